@@ -149,6 +149,11 @@ SIGNATURES: dict[str, tuple] = {
     "difflet_rocm_rms_norm_channels": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp, _f32,
                                               _i32, _vp]),
     "difflet_rocm_rows_to_planes": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _f32, _f32, _vp]),
+    "difflet_rocm_rms_norm_quant": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                           _i32, _i64, _i64, _vp, _i32, _f32, _i32, _vp]),
+    "difflet_rocm_rope_axes": (_i32, [_vp, _vp, _i64p, _i64p, _i64, _vp, _vp, _i64p, _i64p, _i64,
+                                      _i32, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _i64, _vp,
+                                      _vp, _i32, _vp]),
 }
 
 _lib = None

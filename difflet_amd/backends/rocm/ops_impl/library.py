@@ -296,4 +296,58 @@ def _(x, cos, sin, law):
     return x.new_empty(x.shape)
 
 
-__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "rms_norm", "rope"]
+# ---------------------------------------------------------------------------- packed requests
+def _rms_norm_quant_impl(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
+                         eps: float, mx: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """difflet_rocm_rms_norm_quant on x [rows, dim]: (codes, scales, x + residual, which is empty
+    without a residual)."""
+    q, s, h = kernels.rms_norm_quant(x, weight, eps, residual=residual, mx=mx)
+    return q, s, x.new_empty(0) if residual is None else h
+
+
+def _rms_norm_quant_fake(x, weight, residual, eps, mx):
+    rows, dim = x.shape
+    scales = (x.new_empty((rows, dim // 32), dtype=torch.uint8) if mx
+              else x.new_empty((rows,), dtype=torch.float32))
+    return (x.new_empty((rows, dim), dtype=torch.float8_e4m3fn), scales,
+            x.new_empty(0 if residual is None else (rows, dim)))
+
+
+_rms_norm_quant_op = torch.library.custom_op("difflet_rocm::rms_norm_quant", _rms_norm_quant_impl,
+                                             mutates_args=())
+_rms_norm_quant_op.register_fake(_rms_norm_quant_fake)
+_rms_norm_quant_infer = _infer_twin(_rms_norm_quant_op, _rms_norm_quant_impl, _rms_norm_quant_fake)
+
+
+def rms_norm_quant(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float,
+                   mx: bool) -> tuple[Tensor, Tensor, Tensor]:
+    if _inference(x, weight, residual):
+        return _rms_norm_quant_infer.redispatch(_DEVICE, x, weight, residual, eps, mx)
+    return _rms_norm_quant_op(x, weight, residual, eps, mx)
+
+
+def _rope_axes_impl(q: Tensor, k: Optional[Tensor], positions: Tensor, axes: list[int],
+                    theta: float, halves: bool, shared: bool) -> tuple[Tensor, Tensor]:
+    """difflet_rocm_rope_axes on q [B, S, H, D] and k (its output empty without one)."""
+    qo, ko = kernels.rope_axes(q, k, positions, axes, theta=theta, halves=halves, shared=shared)
+    return qo, q.new_empty(0) if ko is None else ko
+
+
+def _rope_axes_fake(q, k, positions, axes, theta, halves, shared):
+    return q.new_empty(q.shape), q.new_empty(0 if k is None else k.shape)
+
+
+_rope_axes_op = torch.library.custom_op("difflet_rocm::rope_axes", _rope_axes_impl, mutates_args=())
+_rope_axes_op.register_fake(_rope_axes_fake)
+_rope_axes_infer = _infer_twin(_rope_axes_op, _rope_axes_impl, _rope_axes_fake)
+
+
+def rope_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, axes: list[int], theta: float,
+              halves: bool, shared: bool) -> tuple[Tensor, Tensor]:
+    if _inference(q, k, positions):
+        return _rope_axes_infer.redispatch(_DEVICE, q, k, positions, axes, theta, halves, shared)
+    return _rope_axes_op(q, k, positions, axes, theta, halves, shared)
+
+
+__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "rms_norm", "rms_norm_quant", "rope",
+           "rope_axes"]

@@ -7,7 +7,10 @@ Outputs are allocated with torch (the library never allocates).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
+import math
 from typing import Sequence
 
 import torch
@@ -1175,3 +1178,152 @@ def rows_to_planes(x: torch.Tensor, channels: int, *, lo: float = float("-inf"),
     check(lib().difflet_rocm_rows_to_planes(_ptr(x), x.stride(0), _dt(x), n, channels, _ptr(y),
                                             float(lo), float(hi), _stream(dev)), "rows_to_planes")
     return y
+
+
+# ------------------------------------------------------------------------ packed requests
+def _current(dev: torch.device):
+    """A context in which dev is the current device, as a launch on its streams needs."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t as [rows, cols] rows that start on 16 bytes, a copy where they do not."""
+    t2 = _rows2d(t, name)
+    if t2.stride(0) % 8 or t2.data_ptr() % 16:
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def _writable_rows(t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, name: str) -> None:
+    if t.dtype != dtype or t.shape != (rows, cols) or (cols > 1 and t.stride(1) != 1) or \
+            t.data_ptr() % 16 or (rows > 1 and (t.stride(0) < cols or t.stride(0) % 8)):
+        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] with rows that start on 16 bytes "
+                         "and do not overlap")
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
+                   residual: torch.Tensor | None = None, mx: bool = False,
+                   hidden: torch.Tensor | None = None
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """RMSNorm of h = x + residual over the last dim, rounded once to e4m3: (codes float8_e4m3fn
+    [rows, dim], scales, h in x's dtype [rows, dim], x itself without a residual). Scales: fp32
+    [rows], or with mx E8M0 uint8 [rows, dim / 32], codes and blocks in swizzle order. hidden: where
+    to write h (x and residual may be given). dim a multiple of 8 (mx: 128), at most 16384."""
+    dev = _on_gpu(x, weight, residual, hidden)
+    if x.dtype not in FLOAT_DTYPES:
+        raise TypeError(f"rms_norm_quant: x must be bf16, fp16 or fp32, got {x.dtype}")
+    dim = x.shape[-1]
+    if weight is not None:
+        if weight.dtype not in FLOAT_DTYPES:
+            raise TypeError(f"rms_norm_quant: weight must be bf16, fp16 or fp32, got {weight.dtype}")
+        if weight.shape != (dim,):
+            raise ValueError(f"rms_norm_quant: weight must be [{dim}], got {tuple(weight.shape)}")
+        if weight.stride(0) != 1 or weight.data_ptr() % 16:
+            weight = weight.clone(memory_format=torch.contiguous_format)
+    x2 = _rows16(x, "rms_norm_quant")
+    rows = x2.shape[0]
+    r2 = None
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError(f"rms_norm_quant: residual must be {x.dtype} {tuple(x.shape)}, got "
+                             f"{residual.dtype} {tuple(residual.shape)}")
+        r2 = _rows16(residual, "rms_norm_quant")
+        if hidden is None:
+            hidden = torch.empty((rows, dim), dtype=x.dtype, device=dev)
+        else:
+            _writable_rows(hidden, rows, dim, x.dtype, "rms_norm_quant: hidden")
+    elif hidden is not None:
+        raise ValueError("rms_norm_quant: hidden is written where a residual is added")
+    q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=dev)
+    s = torch.empty((rows, dim // 32) if mx else (rows,),
+                    dtype=torch.uint8 if mx else torch.float32, device=dev)
+    with _current(dev):
+        check(lib().difflet_rocm_rms_norm_quant(
+            _ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(hidden),
+            0 if hidden is None else max(hidden.stride(0), dim), _ptr(q), dim, _ptr(s),
+            dim // 32 if mx else 0, _dt(x), rows, dim, _ptr(weight),
+            _lib.F32 if weight is None else _dt(weight), float(eps), int(mx), _stream(dev)),
+            "rms_norm_quant")
+    return q, s, x2 if hidden is None else hidden
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_pairs(axes: tuple, theta: float, shared: bool):
+    """Turns per position and axis of every rotated pair, as host arrays."""
+    turns, axis, total = [], [], sum(axes)
+    for a, d in enumerate(axes):
+        for j in range(d // 2):
+            e = 2.0 * (len(axis) if shared else j) / (total if shared else d)
+            turns.append(theta ** -e / (2.0 * math.pi))
+            axis.append(a)
+    return (ctypes.c_double * len(turns))(*turns), (ctypes.c_uint8 * len(axis))(*axis)
+
+
+_POSITIONS = {torch.float32: _lib.F32, torch.int32: _lib.I32, torch.int64: -1}
+
+
+def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
+              axes: Sequence[int], *, theta: float = 10000.0, halves: bool = False,
+              shared: bool = False, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None
+              ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary embedding of q [batch, seq, heads, dim] and k (heads of its own, or None) from
+    positions [batch or 1, seq, len(axes)] (int32, int64 or fp32): axis a turns axes[a] channels.
+    q_out, k_out: where to write (the inputs may be given); new contiguous tensors without."""
+    dev = _on_gpu(q, k, positions, q_out, k_out)
+    axes = tuple(int(d) for d in axes)
+    if not 1 <= len(axes) <= 8 or any(d < 2 or d % 2 for d in axes):
+        raise ValueError(f"rope_axes: 1 to 8 axes of an even number of channels each, got {axes}")
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"rope_axes: theta must be positive, got {theta}")
+    if q.dim() != 4 or q.dtype not in FLOAT_DTYPES:
+        raise ValueError(f"rope_axes: q must be a bf16, fp16 or fp32 [batch, seq, heads, dim], got "
+                         f"{q.dtype} {tuple(q.shape)}")
+    b, s, _, d = q.shape
+    if sum(axes) > d:
+        raise ValueError(f"rope_axes: axes {axes} turn more than the head's {d} channels")
+    if sum(axes) > 256:
+        raise NotImplementedError(f"rope_axes: axes {axes} turn more than 256 channels")
+    if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != (b, s)
+                          or k.shape[3] != d):
+        raise ValueError(f"rope_axes: k must be {q.dtype} [{b}, {s}, heads, {d}], got {k.dtype} "
+                         f"{tuple(k.shape)}")
+    if positions.dtype not in _POSITIONS:
+        raise TypeError(f"rope_axes: positions must be int32, int64 or fp32, got {positions.dtype}")
+    if positions.dim() != 3 or positions.shape[0] not in (1, b) or \
+            positions.shape[1:] != (s, len(axes)):
+        raise ValueError(f"rope_axes: positions must be [{b} or 1, {s}, {len(axes)}], got "
+                         f"{tuple(positions.shape)}")
+    positions = positions.contiguous()
+
+    def prepared(t, out, name):
+        if t is None:
+            if out is not None:
+                raise ValueError(f"rope_axes: {name} without its input")
+            return None, None
+        t = t if t.stride(3) == 1 or d == 1 else t.contiguous()
+        if out is None:
+            return t, torch.empty(t.shape, dtype=t.dtype, device=dev)
+        if out.dtype != t.dtype or out.shape != t.shape or (d > 1 and out.stride(3) != 1) or any(
+                n > 1 and st < d for n, st in zip(out.shape[:3], out.stride()[:3])):
+            raise ValueError(f"rope_axes: {name} must be {t.dtype} {tuple(t.shape)} with heads that "
+                             "are contiguous and do not overlap")
+        return t, out
+
+    q, q_out = prepared(q, q_out, "q_out")
+    k, k_out = prepared(k, k_out, "k_out")
+    turns, axis = _rope_pairs(axes, float(theta), bool(shared))
+    args = []
+    for t, o in ((q, q_out), (k, k_out)):
+        if t is None:
+            args += [None, None, None, None, 0]
+        else:
+            args += [_ptr(t), _ptr(o), _arr(t.stride()[:3]), _arr(o.stride()[:3]), t.shape[2]]
+    with _current(dev):
+        check(lib().difflet_rocm_rope_axes(
+            *args, _dt(q), b, s, d, _ptr(positions), _POSITIONS[positions.dtype],
+            positions.stride(0) if positions.shape[0] > 1 else 0, len(axes), sum(axes) // 2, turns,
+            axis, int(halves), _stream(dev)), "rope_axes")
+    return q_out, k_out

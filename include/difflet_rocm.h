@@ -584,6 +584,44 @@ int difflet_rocm_rows_to_planes(const void* x, int64_t ld, int dtype, int64_t n,
                                 int64_t channels, void* out, float lo, float hi,
                                 difflet_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators over the packed rows of several requests. Where requests are told apart, `starts`
+ * holds requests + 1 int32 row numbers on the device: request i has rows [starts[i],
+ * starts[i + 1]). They are read by the kernels only, so a captured graph follows their values;
+ * values out of order or past the tensor are clamped, never followed.
+ * ---------------------------------------------------------------------------------------- */
+
+/* h = x + residual (fp32; residual NULL: h = x), y = h / sqrt(mean(h^2) + eps) * weight (NULL: 1),
+ * and y rounded once to e4m3 codes: mx == 0 with fp32 scales [rows] by the per-row law of
+ * difflet_rocm_quantize_fp8_rowwise, mx != 0 with E8M0 scales [rows][dim / 32] (row stride lds) in
+ * the swizzle order of difflet_rocm_quantize_mxfp8. hidden (with a residual; may be NULL, x or the
+ * residual): h rounded to x's type. x, residual and hidden of `dtype` (F32, BF16, F16), rows of
+ * strides ldx, ldr, ldh (multiples of 8, 16-byte aligned); weight [dim] of weight_dtype; dim a
+ * multiple of 8 (MX: 128), at most 16384. A row (MX: a block) whose y holds a NaN has NaN codes
+ * and a NaN scale. */
+int difflet_rocm_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                void* hidden, int64_t ldh, uint8_t* codes, int64_t ldq,
+                                void* scales, int64_t lds, int dtype, int64_t rows, int64_t dim,
+                                const void* weight, int weight_dtype, float eps, int mx,
+                                difflet_stream_t stream);
+
+/* Rotary embedding of q and k (either may have no heads) from positions: pair p of every head turns
+ * by positions[b][s][pair_axis[p]] * turns[p] full turns (turns and pair_axis: host arrays of
+ * `pairs` <= 128 entries, read before the call returns), the product in fp64. Pair p is channels
+ * (2 p, 2 p + 1), with halves != 0 (p, pairs + p); channels from 2 pairs on are copied. q, k and
+ * outputs: [batch][seq][heads][head_dim] by strides {batch, seq, head}; an output may be its
+ * input, with the same strides, and overlaps nothing else. positions: [batch][seq][axes], rows of
+ * a batch element contiguous, elements positions_batch_stride apart (0: one for all); F32, I32 or
+ * -1 for int64. */
+int difflet_rocm_rope_axes(const void* q, void* q_out, const int64_t* q_strides,
+                           const int64_t* q_out_strides, int64_t q_heads, const void* k,
+                           void* k_out, const int64_t* k_strides, const int64_t* k_out_strides,
+                           int64_t k_heads, int dtype, int64_t batch, int64_t seq,
+                           int64_t head_dim, const void* positions, int positions_dtype,
+                           int64_t positions_batch_stride, int64_t axes, int64_t pairs,
+                           const double* turns, const uint8_t* pair_axis, int halves,
+                           difflet_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

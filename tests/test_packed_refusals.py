@@ -1,0 +1,77 @@
+"""What the operators over packed requests refuse, before any device work (no GPU needed)."""
+
+import ctypes
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+def test_rms_norm_quantized_refusals():
+    from difflet_amd.backends.rocm.ops_impl.norm import rms_norm_quantized as f
+
+    x = torch.zeros(2, 256, dtype=BF16)
+    with pytest.raises(ValueError, match="format"):
+        f(x, None, 1e-6, format="fp4")
+    with pytest.raises(ValueError, match="device"):
+        f(x, None, 1e-6)
+    m = torch.zeros(2, 256, dtype=BF16, device="meta")
+    with pytest.raises(ValueError, match="device"):
+        f(m, None, 1e-6)
+
+
+def _rms(lib, **kw):
+    a = dict(x=16, ldx=256, residual=None, ldr=0, hidden=None, ldh=0, codes=16, ldq=256, scales=16,
+             lds=8, dtype=1, rows=1, dim=256, weight=None, wdt=0, eps=1e-6, mx=0)
+    a.update(kw)
+    return lib.difflet_rocm_rms_norm_quant(*a.values(), None)
+
+
+def test_rms_norm_quant_entry_point_refusals():
+    from difflet_amd import _lib
+
+    lib = _lib.load()
+    assert _rms(lib, rows=0) == _lib.OK
+    for bad in (dict(dim=12), dict(dim=0), dict(dim=136, mx=1), dict(rows=-1), dict(dtype=3),
+                dict(x=None), dict(codes=None), dict(scales=None), dict(hidden=16),
+                dict(ldx=255), dict(ldq=248), dict(x=8), dict(codes=12), dict(weight=16, wdt=5),
+                dict(mx=1, lds=7), dict(residual=16, ldr=4), dict(residual=16, hidden=16, ldh=128)):
+        assert _rms(lib, **bad) == _lib.EINVAL, bad
+    assert _rms(lib, dim=16392, ldx=16392, ldq=16392) == _lib.EUNSUPPORTED
+
+
+def test_rope_axes_refusals():
+    from difflet_amd import kernels
+    from difflet_amd.backends.rocm.ops_impl.embeddings import apply_rotary_axes as f
+
+    q, pos = torch.zeros(4, 2, 64), torch.zeros(4, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="layout"):
+        f(q, None, pos, (64,), layout="pairs")
+    with pytest.raises(ValueError, match="device"):
+        f(q, None, pos, (64,))
+    with pytest.raises(ValueError, match="device"):
+        kernels.rope_axes(q[None], None, pos[None], (64,))
+
+
+def _rope(lib, **kw):
+    st = (ctypes.c_int64 * 3)(128, 128, 64)
+    a = dict(q=16, qo=16, qs=st, qos=st, qh=2, k=None, ko=None, ks=None, kos=None, kh=0, dtype=1,
+             batch=1, seq=1, dim=64, pos=16, pdt=5, pbs=0, axes=1, pairs=32,
+             turns=(ctypes.c_double * 128)(), axis=(ctypes.c_uint8 * 128)(), halves=0)
+    a.update(kw)
+    return lib.difflet_rocm_rope_axes(*a.values(), None)
+
+
+def test_rope_axes_entry_point_refusals():
+    from difflet_amd import _lib
+
+    lib = _lib.load()
+    assert _rope(lib, seq=0) == _lib.OK
+    assert _rope(lib, qh=0) == _lib.OK
+    ones = (ctypes.c_uint8 * 128)(*[1] * 128)
+    for bad in (dict(dim=0), dict(axes=0), dict(axes=9), dict(pairs=0), dict(pairs=33),
+                dict(pairs=129, dim=512), dict(turns=None), dict(axis=None), dict(axis=ones),
+                dict(dtype=3), dict(pdt=1), dict(q=None), dict(qo=None), dict(qs=None),
+                dict(kh=1), dict(pos=None), dict(batch=-1)):
+        assert _rope(lib, **bad) == _lib.EINVAL, bad
