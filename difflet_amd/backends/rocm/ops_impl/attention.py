@@ -89,6 +89,37 @@ def cross_attention(q, k, v, *, scale: float | None = None, attention_mask=None,
     return attention(q, k, v, scale=scale, causal=False, attention_mask=attention_mask, **kwargs)
 
 
+def packed_cross_attention(q, k, v, q_starts, k_starts, *, scale: float | None = None):
+    """Cross attention of several requests packed behind one another, each to the states of its own
+    encoder: rows [q_starts[i], q_starts[i + 1]) of q [rows, heads, dim] attend to states
+    [k_starts[i], k_starts[i + 1]) of k and v [states, key heads, dim].
+
+    heads is a multiple of the key heads (query head h reads key head h // (heads // key heads)).
+    bf16 or fp16, any strides with a contiguous last dim, dim up to 128 (zero-padded to 64 or 128 as
+    in attention()); ``scale=None`` means 1.0. The starts are int32 tensors on the device, requests
+    + 1 of them, not decreasing; the host never reads them, so a captured graph follows new lengths
+    in the same tensors. A request without states has zero rows, as have rows of no request."""
+    for t in (q, k, v, q_starts, k_starts):
+        if t.device.type != "cuda":
+            raise ValueError(f"rocm attention takes device tensors, got one on {t.device}")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"rocm packed attention runs bf16 / fp16; got {q.dtype}")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"packed attention takes q [rows, heads, dim], k and v [states, key heads, "
+                         f"dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v dtypes differ: {q.dtype}, {k.dtype}, {v.dtype}")
+    if not (q.shape[-1] == k.shape[-1] == v.shape[-1]):
+        raise ValueError(f"q, k, v head dims differ: {q.shape[-1]}, {k.shape[-1]}, {v.shape[-1]}")
+    scale = 1.0 if scale is None else float(scale)
+    d = q.shape[-1]
+    dk = kernel_head_dim(d)
+    if dk != d:
+        q, k, v = (pad_head_dim(t, dk) for t in (q, k, v))
+        return library.packed_attention(q, k, v, q_starts, k_starts, scale)[..., :d]
+    return library.packed_attention(q, k, v, q_starts, k_starts, scale)
+
+
 def _require_cp1(what: str):
     from difflet_amd.backends.rocm.ops_impl import collectives
 
@@ -167,6 +198,7 @@ __all__ = [
     "cross_attention",
     "joint_ring_attention",
     "joint_ulysses_attention",
+    "packed_cross_attention",
     "ring_attention",
     "ulysses_attention",
 ]

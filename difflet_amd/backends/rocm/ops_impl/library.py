@@ -349,5 +349,29 @@ def rope_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, axes: list[int]
     return _rope_axes_op(q, k, positions, axes, theta, halves, shared)
 
 
-__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "rms_norm", "rms_norm_quant", "rope",
-           "rope_axes"]
+def _packed_attention_impl(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts: Tensor,
+                           scale: float) -> Tensor:
+    """difflet_rocm_packed_attention: [rows, heads, dim] of packed requests."""
+    return kernels.packed_attention(q, k, v, q_starts, k_starts, scale=scale)
+
+
+def _packed_attention_fake(q, k, v, q_starts, k_starts, scale):
+    return q.new_empty(q.shape)
+
+
+_packed_attention_op = torch.library.custom_op("difflet_rocm::packed_attention",
+                                               _packed_attention_impl, mutates_args=())
+_packed_attention_op.register_fake(_packed_attention_fake)
+_packed_attention_infer = _infer_twin(_packed_attention_op, _packed_attention_impl,
+                                      _packed_attention_fake)
+
+
+def packed_attention(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts: Tensor,
+                     scale: float) -> Tensor:
+    if _inference(q, k, v, q_starts, k_starts):
+        return _packed_attention_infer.redispatch(_DEVICE, q, k, v, q_starts, k_starts, scale)
+    return _packed_attention_op(q, k, v, q_starts, k_starts, scale)
+
+
+__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "packed_attention", "rms_norm",
+           "rms_norm_quant", "rope", "rope_axes"]

@@ -1327,3 +1327,65 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
             positions.stride(0) if positions.shape[0] > 1 else 0, len(axes), sum(axes) // 2, turns,
             axis, int(halves), _stream(dev)), "rope_axes")
     return q_out, k_out
+
+
+def _starts(t: torch.Tensor, requests: int | None, name: str) -> int:
+    """Checks row numbers of packed requests, int32 [requests + 1]; the number of requests."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.dim() != 1 or t.shape[0] < 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (
+            requests is not None and t.shape[0] != requests + 1):
+        want = "requests" if requests is None else requests
+        raise ValueError(f"{name} must be a contiguous [{want} + 1], got {tuple(t.shape)}")
+    return t.shape[0] - 1
+
+
+def _heads16(t: torch.Tensor) -> torch.Tensor:
+    """t [rows, heads, dim] with contiguous heads that start on 16 bytes, a copy where they do not."""
+    ok = (t.shape[2] == 1 or t.stride(2) == 1) and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or st % 8 == 0 for n, st in zip(t.shape[:2], t.stride()[:2]))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_head(t: torch.Tensor):
+    return _arr([st if n > 1 else 0 for n, st in zip(t.shape[:2], t.stride()[:2])])
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor,
+                     k_starts: torch.Tensor, *, scale: float,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T scale) v of packed requests: q [rows, heads, dim], k and v [states, key heads,
+    dim] (heads a multiple of them), bf16 or fp16, dim 64 or 128. Request i has rows q_starts[i] ..
+    q_starts[i + 1] - 1 and states k_starts[i] .. k_starts[i + 1] - 1 (int32 on the device, not read
+    by the host). A request without states has zero rows; rows of no request are zero, in a given
+    `out` left as they are."""
+    dev = _on_gpu(q, k, v, q_starts, k_starts, out)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"packed_attention: q [rows, heads, dim] with k and v [states, key heads, "
+                         f"dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError(f"packed_attention: dtypes differ: {q.dtype}, {k.dtype}, {v.dtype}")
+    rows, h, d = q.shape
+    hk = k.shape[1]
+    if hk == 0 or h == 0 or h % hk:
+        raise ValueError(f"packed_attention: {h} heads over {hk} key heads")
+    n = _starts(q_starts, None, "packed_attention: q_starts")
+    _starts(k_starts, n, "packed_attention: k_starts")
+    if out is None:
+        o = torch.empty((rows, h, d), dtype=q.dtype, device=dev)
+    else:
+        o = out
+        if o.dtype != q.dtype or o.shape != q.shape or o.stride(2) != 1 or o.data_ptr() % 8 or any(
+                m > 1 and (st < d or st % 4) for m, st in zip(o.shape[:2], o.stride()[:2])):
+            raise ValueError(f"packed_attention: out must be {q.dtype} {tuple(q.shape)} with heads "
+                             "that start on 8 bytes and do not overlap")
+    q, k, v = _heads16(q), _heads16(k), _heads16(v)
+    with _current(dev):
+        nbytes = lib().difflet_rocm_packed_attention_workspace_bytes(rows, k.shape[0], n, hk,
+                                                                     h // hk, d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        check(lib().difflet_rocm_packed_attention(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(o), _dt(q), rows, k.shape[0], hk, h // hk, d,
+            _row_head(q), _row_head(k), _row_head(v), _row_head(o), _ptr(q_starts), _ptr(k_starts),
+            n, float(scale), int(out is None), _ptr(ws), nbytes, _stream(dev)), "packed_attention")
+    return o

@@ -622,6 +622,27 @@ int difflet_rocm_rope_axes(const void* q, void* q_out, const int64_t* q_strides,
                            const double* turns, const uint8_t* pair_axis, int halves,
                            difflet_stream_t stream);
 
+/* Cross attention over packed requests: rows [q_starts[i], q_starts[i + 1]) of q attend to keys
+ * [k_starts[i], k_starts[i + 1]), out = softmax(q k^T * scale) v, softmax in fp32. q, o: [rows_q]
+ * [kv_heads * group][head_dim] by strides {row, head}, k, v: [rows_k][kv_heads][head_dim]; query
+ * head h reads key head h / group. BF16 or F16, head_dim 64 or 128, any finite scale. A request
+ * without keys has zero rows. Rows of no request are zero with zero_rest != 0 and not written
+ * without. Rows and heads of q, k, v start on 16 bytes, of o on 8; o overlaps nothing. Few query
+ * tiles cut each request's keys into pieces when the workspace
+ * (difflet_rocm_packed_attention_workspace_bytes, this call's alone, 256-byte aligned, any contents)
+ * is there, joined in order; without it the keys stay whole. */
+int64_t difflet_rocm_packed_attention_workspace_bytes(int64_t rows_q, int64_t rows_k,
+                                                      int64_t requests, int64_t kv_heads,
+                                                      int64_t group, int64_t head_dim);
+int difflet_rocm_packed_attention(const void* q, const void* k, const void* v, void* o, int dtype,
+                                  int64_t rows_q, int64_t rows_k, int64_t kv_heads, int64_t group,
+                                  int64_t head_dim, const int64_t* q_strides,
+                                  const int64_t* k_strides, const int64_t* v_strides,
+                                  const int64_t* o_strides, const int32_t* q_starts,
+                                  const int32_t* k_starts, int64_t requests, float scale,
+                                  int zero_rest, void* workspace, int64_t workspace_bytes,
+                                  difflet_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

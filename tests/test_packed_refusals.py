@@ -75,3 +75,42 @@ def test_rope_axes_entry_point_refusals():
                 dict(dtype=3), dict(pdt=1), dict(q=None), dict(qo=None), dict(qs=None),
                 dict(kh=1), dict(pos=None), dict(batch=-1)):
         assert _rope(lib, **bad) == _lib.EINVAL, bad
+
+
+def test_packed_cross_attention_refusals():
+    from difflet_amd import kernels
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention as f
+
+    q, s = torch.zeros(4, 2, 64, dtype=BF16), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="device"):
+        f(q, q, q, s, s)
+    with pytest.raises(ValueError, match="device"):
+        kernels.packed_attention(q, q, q, s, s, scale=1.0)
+
+
+def _attn(lib, **kw):
+    st = (ctypes.c_int64 * 2)(128, 64)
+    a = dict(q=16, k=16, v=16, o=16, dtype=1, rq=1, rk=1, hk=2, g=1, d=64, qs=st, ks=st, vs=st,
+             os=st, qst=16, kst=16, n=1, scale=1.0, zero=1, ws=None, wb=0)
+    a.update(kw)
+    return lib.difflet_rocm_packed_attention(*a.values(), None)
+
+
+def test_packed_attention_entry_point_refusals():
+    from difflet_amd import _lib
+
+    lib = _lib.load()
+    assert _attn(lib, rq=0) == _lib.OK
+    odd, far = (ctypes.c_int64 * 2)(124, 64), (ctypes.c_int64 * 2)(1 << 24, 64)
+    back = (ctypes.c_int64 * 2)(-128, 64)
+    for bad in (dict(hk=0), dict(g=0), dict(rq=-1), dict(n=-1), dict(q=None), dict(k=None),
+                dict(o=None), dict(qst=None), dict(kst=None), dict(qs=None), dict(qs=odd),
+                dict(ks=odd), dict(q=8), dict(v=24), dict(o=4), dict(scale=float("inf")),
+                dict(scale=float("nan"))):
+        assert _attn(lib, **bad) == _lib.EINVAL, bad
+    for bad in (dict(dtype=0), dict(d=32), dict(ks=far), dict(vs=back), dict(rq=1 << 31),
+                dict(hk=65537)):
+        assert _attn(lib, **bad) == _lib.EUNSUPPORTED, bad
+    size = lib.difflet_rocm_packed_attention_workspace_bytes
+    assert size(16, 32000, 16, 4, 7, 128) > 0  # single tokens: keys in pieces
+    assert size(40000, 738, 2, 40, 1, 128) == 0 and size(0, 1, 1, 1, 1, 64) == 0
