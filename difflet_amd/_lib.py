@@ -158,6 +158,10 @@ SIGNATURES: dict[str, tuple] = {
     "difflet_rocm_packed_attention": (_i32, [
         _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _vp,
         _vp, _i64, _f32, _i32, _vp, _i64, _vp]),
+    "difflet_rocm_lora_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64]),
+    "difflet_rocm_lora_linear": (_i32, [
+        _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp,
+        _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
 }
 
 _lib = None

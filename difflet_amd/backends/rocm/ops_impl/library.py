@@ -373,5 +373,40 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts
     return _packed_attention_op(q, k, v, q_starts, k_starts, scale)
 
 
-__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "packed_attention", "rms_norm",
-           "rms_norm_quant", "rope", "rope_axes"]
+def _lora_linear_impl(x: Tensor, w: Tensor, w_scale: Optional[Tensor], bias: Optional[Tensor],
+                      down: Tensor, up: Tensor, scale: Tensor, starts: Tensor, ids: Tensor) -> Tensor:
+    """difflet_rocm_lora_linear: y [M, N] bf16 of bf16 x [M, K] and w [N, K] bf16, or e4m3 codes
+    with per-channel fp32 or E8M0 block scales. Widths off the bf16 GEMM's multiples (K 64, N 4)
+    are zero-padded here."""
+    kind = "bf16" if w_scale is None else "mx" if w_scale.dtype == torch.uint8 else "fp8"
+    n, k = w.shape
+    if kind == "bf16" and (k % 64 or n % 4):
+        kp, np_ = -(-k // 64) * 64, -(-n // 4) * 4
+        x, w = F.pad(x, (0, kp - k)), F.pad(w, (0, kp - k, 0, np_ - n))
+        bias = None if bias is None else F.pad(bias, (0, np_ - n))
+        if k % 8:
+            down = F.pad(down, (0, kp - k))
+    y = kernels.lora_linear(kind, x, w, bias, down, up, scale, starts, ids, w_scale=w_scale)
+    return y if y.shape[1] == n else y[:, :n].contiguous()
+
+
+def _lora_linear_fake(x, w, w_scale, bias, down, up, scale, starts, ids):
+    return x.new_empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16)
+
+
+_lora_linear_op = torch.library.custom_op("difflet_rocm::lora_linear", _lora_linear_impl,
+                                          mutates_args=())
+_lora_linear_op.register_fake(_lora_linear_fake)
+_lora_linear_infer = _infer_twin(_lora_linear_op, _lora_linear_impl, _lora_linear_fake)
+
+
+def lora_linear(x: Tensor, w: Tensor, w_scale: Optional[Tensor], bias: Optional[Tensor],
+                down: Tensor, up: Tensor, scale: Tensor, starts: Tensor, ids: Tensor) -> Tensor:
+    if _inference(x, w, w_scale, bias, down, up, scale, starts, ids):
+        return _lora_linear_infer.redispatch(_DEVICE, x, w, w_scale, bias, down, up, scale, starts,
+                                             ids)
+    return _lora_linear_op(x, w, w_scale, bias, down, up, scale, starts, ids)
+
+
+__all__ = ["attention", "fp8_linear", "layer_norm", "linear", "lora_linear", "packed_attention",
+           "rms_norm", "rms_norm_quant", "rope", "rope_axes"]

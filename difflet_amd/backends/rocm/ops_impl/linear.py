@@ -12,6 +12,9 @@ linears, HBM-bound on W), more through the tiled GEMM; fp32 weights (a model loa
 as the T5 encoders' fp32 option) run the fp32 matrix-core GEMM, in fp32 throughout as F.linear
 does. A K or N off the kernel's multiples (64 and 4 for bf16, 4 and 4 for fp32) is zero-padded once
 on the weight (and per call on the input).
+
+lora_linear runs such a weight, or an fp8 linear's, for the packed rows of several requests with a
+low-rank adapter of each request's own.
 """
 
 from __future__ import annotations
@@ -132,6 +135,38 @@ class RowParallelLinear(_RocmLinearBase):
                 f"skip_bias_add={self.skip_bias_add}")
 
 
+def lora_linear(x, weight, bias, down, up, scale, row_starts, adapter, *, weight_scale=None):
+    """``x W^T + b`` for the packed rows of several requests, each with its request's low-rank
+    adapter beside it: ``+ scale[a] (x down[a]^T) up[a]^T`` with a = adapter[i] for rows
+    row_starts[i] .. row_starts[i + 1] - 1 of request i.
+
+    x [..., K] (rows over the leading dims). weight [N, K]: bf16, or an fp8 linear's prepared codes
+    (``FP8Linear.weight_kernel``) with ``weight_scale`` its scales, fp32 [N] or uint8 [N, K / 32];
+    the adapters read the unquantized x. down [adapters, rank, K] and up [adapters, N, rank] bf16 (a
+    smaller adapter's ranks padded with zeros), scale fp32 [adapters]. row_starts int32 [requests +
+    1], not decreasing, and adapter int32 [requests] are read on the device only, so a captured graph
+    follows new requests in the same tensors; an adapter of -1, and rows of no request, have none.
+    The rank values are summed in fp32 and rounded to bf16, the result is rounded once, to x's
+    dtype through bf16."""
+    for t in (x, weight, bias, down, up, scale, row_starts, adapter, weight_scale):
+        if t is not None and t.device.type != "cuda":
+            raise ValueError("rocm linear takes device tensors")
+    if weight_scale is None and weight.dtype != torch.bfloat16:
+        raise NotImplementedError(f"rocm lora_linear runs bf16 weights, or fp8 codes with their "
+                                  f"scales; got {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not chain")
+    n, k = weight.shape
+    if down.dim() != 3 or down.shape[2] != k or up.dim() != 3 or up.shape[1] != n:
+        raise ValueError(f"adapters of this weight are down [adapters, rank, {k}] and up [adapters, "
+                         f"{n}, rank], got {tuple(down.shape)} and {tuple(up.shape)}")
+    x2 = x.reshape(-1, k)
+    b = None if bias is None else bias.detach().to(torch.bfloat16)
+    y = library.lora_linear(x2.to(torch.bfloat16), weight, weight_scale, b, down, up, scale,
+                            row_starts, adapter)
+    return y.reshape(*x.shape[:-1], n).to(x.dtype)
+
+
 class ParallelEmbedding(nn.Embedding):
     """nn.Embedding at tp = 1 (a gather, not on the denoise step's path)."""
 
@@ -141,4 +176,4 @@ class ParallelEmbedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim)
 
 
-__all__ = ["ColumnParallelLinear", "ParallelEmbedding", "RowParallelLinear"]
+__all__ = ["ColumnParallelLinear", "ParallelEmbedding", "RowParallelLinear", "lora_linear"]

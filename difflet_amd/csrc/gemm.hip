@@ -34,6 +34,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "adapters.hpp"
 #include "common.hpp"
 #include "gemm_small.hpp"
 
@@ -124,6 +125,11 @@ struct GemmArgs {
   const float* rope_sin;
 };
 
+// A launch with adapters of packed requests beside the shared weight (adapters.hpp).
+struct GemmLoraArgs : GemmArgs {
+  LoraDev lora;
+};
+
 // KT: K elements per stage, KTB its bytes per row, NSLOT the stages the LDS ring holds. WN:
 // wavefronts along N (two along M). Every type runs 8 wavefronts of 128 x 64 (measured against 4
 // of 128 x 128: +10-20 % for fp8, +0-6 % for bf16, and 128 accumulators leave room for the
@@ -186,8 +192,12 @@ __device__ __forceinline__ f32x16 mfma_mx(const i32x8& w, const i32x8& a, const 
 // SPLIT: the launch uses the split schedule (workgroups may own several tiles or parts of
 // them). Whole-tile launches (SPLIT false, the DiT steps) hold no state across tiles, so the
 // K loop's addressing and the epilogue do not compete for registers with a tile loop.
-template <Elem E, int EPI, int WN, bool QK, bool SPLIT>
-__global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) {
+// LORA: the adapters' stages follow the K loop, run by the tile's first piece; per-row fp8's scales
+// are then applied before them, to each piece's sums, and not in the epilogue.
+template <Elem E, int EPI, int WN, bool QK, bool SPLIT, bool LORA = false>
+__global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
+    const std::conditional_t<LORA, GemmLoraArgs, GemmArgs> args) {
+  constexpr bool SCALED = E == Elem::FP8 && !LORA;  // the epilogue applies the fp8 scales
   constexpr int KT = ElemTraits<E>::KT;
   constexpr int EB = ElemTraits<E>::BYTES;
   constexpr int KTB = ElemTraits<E>::KTB, NSLOT = ElemTraits<E>::NSLOT;
@@ -464,6 +474,64 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
     }
   }
 
+  if constexpr (LORA) {
+    __syncthreads();  // every wave's last fragment reads of the ring are done
+    if constexpr (E == Elem::FP8) {
+      float sa[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + wm * 128 + i * 32 + frow;
+        sa[i] = m < M ? reinterpret_cast<const float*>(P.a_scale)[m] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t n = n0 + wn * WTN + j * 32 + q * 8 + fhalf * 4;
+          const f32x4 wv = n < N ? *reinterpret_cast<const f32x4*>(
+                                       reinterpret_cast<const float*>(P.w_scale) + n)
+                                 : f32x4{};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= sa[i] * wv[e];
+        }
+    }
+    if (kbeg == 0)
+      lora_stages<BM, BN, 128 * WN>(
+          args.lora, (int)m0, (int)n0, lds, lds + (BM + BN) * KTB, [](int r) { return swz8(r); },
+          [&](int ks) {
+            bf16x8 fx[4], fy[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              fx[i] = *reinterpret_cast<const bf16x8*>(
+                  lds + lds_off8(wm * 128 + i * 32 + frow, 2 * ks + fhalf));
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+              fy[j] = *reinterpret_cast<const bf16x8*>(
+                  lds + BM * KTB + lds_off8(wn * WTN + j * 32 + frow, 2 * ks + fhalf));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < TJ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[j], fx[i], acc[i][j], 0, 0, 0);
+          },
+          [&](const int* slot, const uint32_t* bad) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int s = slot[wm * 128 + i * 32 + frow];
+#pragma unroll
+              for (int j = 0; j < TJ; ++j) {
+                const uint32_t bits = s < 0 ? 0u : bad[s * (BN / 32) + ((wn * WTN + j * 32) >> 5)];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if ((bits >> ((e >> 2) * 8 + fhalf * 4 + (e & 3))) & 1u)
+                    acc[i][j][e] = __builtin_nanf("");
+              }
+            }
+          });
+  }
+
   // ---- a tile cut between XCDs c0 .. c1: the last contributor to arrive finishes it.
   // Partial sums move through the workspace with device-scope (sc1) loads and stores, which
   // the L2 of another XCD cannot serve stale; a store is complete (vmcnt) before its workgroup
@@ -599,7 +667,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
     const float* wsc = reinterpret_cast<const float*>(P.w_scale);
     // the 4 row scales (fp8) for the whole tile; a W tile's column vectors while it is stored
     float sa[4] = {1.f, 1.f, 1.f, 1.f};
-    if constexpr (E == Elem::FP8)
+    if constexpr (SCALED)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t m = m0 + wm * 128 + i * 32 + frow;
@@ -619,7 +687,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
           const int64_t n = n0 + wn * WTN + j * 32 + q * 8 + fhalf * 4;
           const bool nok = n < N;
           bv[q] = (P.bias && nok) ? *reinterpret_cast<const u32x2*>(P.bias + n) : u32x2{0u, 0u};
-          if constexpr (E == Elem::FP8)
+          if constexpr (SCALED)
             wv[q] = nok ? *reinterpret_cast<const f32x4*>(wsc + n) : f32x4{};
         }
 #pragma unroll
@@ -632,7 +700,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               v[e] = acc[i][j][q * 4 + e];
-              if constexpr (E == Elem::FP8) v[e] = v[e] * (sa[i] * wv[q][e]);
+              if constexpr (SCALED) v[e] = v[e] * (sa[i] * wv[q][e]);
               v[e] += bf16bits_to_f32(e & 1 ? bv[q][e >> 1] >> 16 : bv[q][e >> 1] & 0xffffu);
               if constexpr (G == 1) v[e] = gelu_tanh(v[e]);
               if constexpr (G == 2) {
@@ -803,7 +871,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
         const int64_t n = n0 + wn * WTN + j * 32 + q * 8 + fhalf * 4;
         const bool nok = n < N;
         bias_v[j][q] = (bias && nok) ? *reinterpret_cast<const u32x2*>(bias + n) : u32x2{0u, 0u};
-        if constexpr (E == Elem::FP8)
+        if constexpr (SCALED)
           ws_v[j][q] = nok ? *reinterpret_cast<const f32x4*>(ws + n) : f32x4{};
         if constexpr (EPI == DIFFLET_EPI_GATE_RESIDUAL) {
           // one gate row per batch element: a wave's 128 rows lie in one batch element, since
@@ -821,7 +889,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
       const bool mok = m < M;
       const int64_t mc = mok ? m : 0;  // clamped row for address formation
       float sa = 1.f;
-      if constexpr (E == Elem::FP8) sa = mok ? reinterpret_cast<const float*>(P.a_scale)[mc] : 0.f;
+      if constexpr (SCALED) sa = mok ? reinterpret_cast<const float*>(P.a_scale)[mc] : 0.f;
       bf16* crow = reinterpret_cast<bf16*>(P.c) + mc * P.ldc;
       u32x2 res_v[4][4];
       if constexpr (EPI == DIFFLET_EPI_GATE_RESIDUAL) {
@@ -843,7 +911,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
   #pragma unroll
           for (int e = 0; e < 4; ++e) {
             v[e] = acc[i][j][q * 4 + e];
-            if constexpr (E == Elem::FP8) v[e] = v[e] * (sa * ws_v[j][q][e]);
+            if constexpr (SCALED) v[e] = v[e] * (sa * ws_v[j][q][e]);
             v[e] += bf16bits_to_f32(e & 1 ? bias_v[j][q][e >> 1] >> 16
                                           : bias_v[j][q][e >> 1] & 0xffffu);
           }
@@ -915,7 +983,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
           const int64_t nc = n0 + wn * WTN + j * 32 + q * 8 + fhalf * 4;
           const bool nok = nc < N;
           bv[q] = (P.bias && nok) ? *reinterpret_cast<const u32x2*>(P.bias + nc) : u32x2{0u, 0u};
-          if constexpr (E == Elem::FP8)
+          if constexpr (SCALED)
             wv[q] = nok ? *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(P.w_scale) + nc)
                         : f32x4{};
         }
@@ -923,7 +991,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
         for (int i = 0; i < 4; ++i) {
           const int r = i * 32 + frow;  // row within the half
           float sa = 1.f;
-          if constexpr (E == Elem::FP8)
+          if constexpr (SCALED)
             sa = mh + r < M ? reinterpret_cast<const float*>(P.a_scale)[mh + r] : 0.f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -932,7 +1000,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(const GemmArgs args) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float v = acc[i][j][q * 4 + e];
-              if constexpr (E == Elem::FP8) v = v * (sa * wv[q][e]);
+              if constexpr (SCALED) v = v * (sa * wv[q][e]);
               y[e] = v + bf16bits_to_f32(e & 1 ? bv[q][e >> 1] >> 16 : bv[q][e >> 1] & 0xffffu);
             }
             *reinterpret_cast<f32x4*>(yt + r * 256 + (((cl >> 2) ^ (r & 63)) << 2)) = y;
@@ -1110,7 +1178,8 @@ template <Elem E>
 static int gemm_launch(const char* name, int nproblems, const difflet_gemm_problem* problems,
                        int64_t n, int64_t k, int epilogue, int64_t act_col_start,
                        void* workspace, int64_t workspace_bytes, const difflet_gemm_qk* qk,
-                       hipStream_t stream, bool own_scratch = false) {
+                       hipStream_t stream, bool own_scratch = false,
+                       const LoraDev* lora = nullptr) {
   constexpr int KT = ElemTraits<E>::KT;
   constexpr int EB = ElemTraits<E>::BYTES;
   DLT_REQUIRE(problems && nproblems >= 1 && nproblems <= MAX_PROBLEMS, DIFFLET_EINVAL,
@@ -1257,7 +1326,7 @@ static int gemm_launch(const char* name, int nproblems, const difflet_gemm_probl
     if (plan.bm > 0) {
       gemm_small(small_elem<E>(), plan, problems[0], n, k, epilogue == DIFFLET_EPI_GATE_RESIDUAL,
                  args.p[0].rows_per_batch, workspace ? (uint8_t*)workspace + SK_CTR_BYTES : nullptr,
-                 stream);
+                 stream, lora);
       return dlt_check_launch(name);
     }
   }
@@ -1275,6 +1344,18 @@ static int gemm_launch(const char* name, int nproblems, const difflet_gemm_probl
                        stream, reinterpret_cast<int*>(workspace), args.sk.S);
     const int st = dlt_check_launch(name);
     if (st != DIFFLET_OK) return st;
+  }
+  if (lora) {  // one problem without an epilogue
+    GemmLoraArgs la = {};
+    static_cast<GemmArgs&>(la) = args;
+    la.lora = *lora;
+    if (split)
+      hipLaunchKernelGGL((gemm_kernel<E, DIFFLET_EPI_NONE, NT, false, true, true>), grid, block, 0,
+                         stream, la);
+    else
+      hipLaunchKernelGGL((gemm_kernel<E, DIFFLET_EPI_NONE, NT, false, false, true>), grid, block, 0,
+                         stream, la);
+    return dlt_check_launch(name);
   }
   auto go = [&](auto epi, auto fused) {
     constexpr int EP = decltype(epi)::value;
@@ -1338,6 +1419,18 @@ extern "C" int64_t difflet_rocm_gemm_scratch_bytes(int kind, int64_t m, int64_t 
                                   : small_plan(SmallElem::F32, m, n, k, cus, cap, 2e30);
   if (p.bm > 0) return p.pieces > 1 ? SK_CTR_BYTES + p.pieces * m * n * 4 : 0;
   return sk.groups > 0 ? sk_workspace_bytes(cus) : 0;
+}
+
+int dlt::gemm_lora(int kind, const difflet_gemm_problem& q, int64_t n, int64_t k, void* workspace,
+                   int64_t workspace_bytes, hipStream_t stream, const LoraDev& lora) {
+  auto run = [&](auto e) {
+    return gemm_launch<decltype(e)::value>("lora_linear", 1, &q, n, k, DIFFLET_EPI_NONE, 0, workspace,
+                                           workspace_bytes, nullptr, stream, true, &lora);
+  };
+  using std::integral_constant;
+  if (kind == 0) return run(integral_constant<Elem, Elem::BF16>{});
+  if (kind == 1) return run(integral_constant<Elem, Elem::FP8>{});
+  return run(integral_constant<Elem, Elem::MX>{});
 }
 
 extern "C" int difflet_rocm_gemm_single(int kind, const void* a, int64_t lda, const void* w,

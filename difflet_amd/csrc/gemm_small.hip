@@ -31,7 +31,9 @@
 // pieces in order and runs the epilogue. Nothing is kept between launches and nobody waits, so
 // any scratch buffer serves, on any stream and under graph capture.
 #include <algorithm>
+#include <type_traits>
 
+#include "adapters.hpp"
 #include "common.hpp"
 #include "gemm_small.hpp"
 
@@ -52,6 +54,13 @@ struct SmallArgs {
   int pieces, piece_stages;  // K pieces per tile, stages per piece (the last may be shorter)
   float* part;               // fp32 sums [pieces][m][n] (pieces > 1)
 };
+
+// A launch with adapters of packed requests beside the shared weight (adapters.hpp): their stages
+// follow piece 0's K loop. Per-row fp8's scales are applied before them, to every piece's sums.
+struct SmallLoraArgs : SmallArgs {
+  LoraDev lora;
+};
+template <bool LORA> using SmallArgsOf = std::conditional_t<LORA, SmallLoraArgs, SmallArgs>;
 
 // direct-to-LDS load of 16 bytes per lane (as attention.hip's dma16, with a scalar offset):
 // untracked by the compiler, waited for by the K loop's own vmcnt
@@ -77,7 +86,8 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ int swz8s(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 // v (8 columns from n on of row m, fp32 sums) through the epilogue into C: the math of gemm.hip.
-template <SmallElem E, bool GATE>
+// SCALED: per-row fp8's scales are still to be applied.
+template <SmallElem E, bool GATE, bool SCALED = E == SmallElem::FP8>
 __device__ __forceinline__ void small_store8(const SmallArgs& a, int64_t m, int64_t n, float* v) {
   if (n >= a.n) return;
   const bool full = n + 8 <= a.n;  // n % 4 == 0: a chunk is full or half full
@@ -112,7 +122,7 @@ __device__ __forceinline__ void small_store8(const SmallArgs& a, int64_t m, int6
       o[4 + e] = bf16bits_to_f32(e & 1 ? hi[e >> 1] >> 16 : hi[e >> 1] & 0xffffu);
     }
   };
-  if constexpr (E == SmallElem::FP8) {
+  if constexpr (SCALED) {
     const float* ws = reinterpret_cast<const float*>(a.w_scale) + n;
     const float sa = reinterpret_cast<const float*>(a.a_scale)[m];
     const f32x4 w0 = *reinterpret_cast<const f32x4*>(ws);
@@ -145,9 +155,10 @@ __device__ __forceinline__ void small_store8(const SmallArgs& a, int64_t m, int6
   }
 }
 
-template <SmallElem E, int BM, int BN, int NSLOT, bool GATE>
+template <SmallElem E, int BM, int BN, int NSLOT, bool GATE, bool LORA = false>
 __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
-    const SmallArgs args) {
+    const SmallArgsOf<LORA> args) {
+  constexpr bool SCALED = E == SmallElem::FP8 && !LORA;
   constexpr bool F32 = E == SmallElem::F32;
   constexpr int EB = F32 ? 4 : E == SmallElem::BF16 ? 2 : 1;
   constexpr int NW = BN == 64 ? 4 : 8, NT = NW * 64;  // wavefronts, threads
@@ -370,6 +381,63 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
   // BN / 8 lanes per row take 8 columns each (whole lines per store)
   wait_vm<0>();
   __syncthreads();
+  if constexpr (LORA) {
+    static_assert(NSLOT * SLOT >= SLOT + LORA_BOOK_BYTES, "the adapters' bookkeeping fits the ring");
+    if constexpr (E == SmallElem::FP8) {
+      float sa[4];
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int m = m0 + wm * WTM + i * 32 + frow;
+        sa[i] = m < M ? reinterpret_cast<const float*>(args.a_scale)[m] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + wn * WTN + j * 32 + q * 8 + fhalf * 4;
+          const f32x4 wv = n < N ? *reinterpret_cast<const f32x4*>(
+                                       reinterpret_cast<const float*>(args.w_scale) + n)
+                                 : f32x4{};
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= sa[i] * wv[e];
+        }
+    }
+    if (piece == 0)
+      lora_stages<BM, BN, NT>(
+          args.lora, m0, n0, lds, lds + SLOT, [](int r) { return swz8s(r); },
+          [&](int ks) {
+            bf16x8 fx[4], fy[4];
+            auto at = [&](int r) { return r * 128 + (((2 * ks + fhalf) ^ swz8s(r)) << 4); };
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+              fx[i] = *reinterpret_cast<const bf16x8*>(lds + at(wm * WTM + i * 32 + frow));
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+              fy[j] = *reinterpret_cast<const bf16x8*>(lds + BM * 128 + at(wn * WTN + j * 32 + frow));
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+              for (int j = 0; j < TJ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[j], fx[i], acc[i][j], 0, 0, 0);
+          },
+          [&](const int* slot, const uint32_t* bad) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+              const int s = slot[wm * WTM + i * 32 + frow];
+#pragma unroll
+              for (int j = 0; j < TJ; ++j) {
+                const uint32_t bits = s < 0 ? 0u : bad[s * (BN / 32) + ((wn * WTN + j * 32) >> 5)];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if ((bits >> ((e >> 2) * 8 + fhalf * 4 + (e & 3))) & 1u)
+                    acc[i][j][e] = __builtin_nanf("");
+              }
+            }
+          });
+    __syncthreads();
+  }
   float* tile = reinterpret_cast<float*>(lds);
   constexpr int CM = BN / 4 < 32 ? BN / 4 - 1 : 31;
 #pragma unroll
@@ -402,13 +470,13 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
       if (n + 4 < N) *reinterpret_cast<f32x4*>(p + 4) = y1;
     } else {
       float v[8] = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
-      small_store8<E, GATE>(args, m, n, v);
+      small_store8<E, GATE, SCALED>(args, m, n, v);
     }
   }
 }
 
 // C = epilogue(sum of the K pieces in order), 8 columns per thread.
-template <SmallElem E, bool GATE>
+template <SmallElem E, bool GATE, bool SCALED = E == SmallElem::FP8>
 __global__ __launch_bounds__(256) void gemm_small_reduce(const SmallArgs args) {
   const int chunks = (args.n + 7) >> 3;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -428,7 +496,7 @@ __global__ __launch_bounds__(256) void gemm_small_reduce(const SmallArgs args) {
       v[4 + e] += y[e];
     }
   }
-  small_store8<E, GATE>(args, m, n, v);
+  small_store8<E, GATE, SCALED>(args, m, n, v);
 }
 
 // Estimated times on MI355X, in us, from sweeps over 16 to 3000 rows of the layers' widths:
@@ -479,8 +547,8 @@ SmallPlan small_plan(SmallElem e, int64_t m, int64_t n, int64_t k, int cus, int6
   return best;
 }
 
-template <SmallElem E, bool GATE>
-static void launch_small(const SmallArgs& a, const SmallPlan& p, hipStream_t s) {
+template <SmallElem E, bool GATE, bool LORA = false>
+static void launch_small(const SmallArgsOf<LORA>& a, const SmallPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.pieces)), block(512);
   if constexpr (E == SmallElem::F32) {
     if (p.bm == 64)
@@ -489,21 +557,23 @@ static void launch_small(const SmallArgs& a, const SmallPlan& p, hipStream_t s) 
       hipLaunchKernelGGL((gemm_small_kernel<E, 128, 128, 2, GATE>), grid, block, 0, s, a);
   } else {
     if (p.bm == 64)
-      hipLaunchKernelGGL((gemm_small_kernel<E, 64, 128, 5, GATE>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((gemm_small_kernel<E, 64, 128, 5, GATE, LORA>), grid, block, 0, s, a);
     else if (p.bm == 128)
-      hipLaunchKernelGGL((gemm_small_kernel<E, 128, 128, 4, GATE>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((gemm_small_kernel<E, 128, 128, 4, GATE, LORA>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((gemm_small_kernel<E, 256, 128, 3, GATE>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((gemm_small_kernel<E, 256, 128, 3, GATE, LORA>), grid, block, 0, s, a);
   }
   if (p.pieces > 1) {
     const int64_t chunks = (int64_t)a.m * ((a.n + 7) / 8);
-    hipLaunchKernelGGL((gemm_small_reduce<E, GATE>), dim3((unsigned)((chunks + 255) / 256)),
-                       dim3(256), 0, s, a);
+    hipLaunchKernelGGL((gemm_small_reduce<E, GATE, E == SmallElem::FP8 && !LORA>),
+                       dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, s,
+                       static_cast<const SmallArgs&>(a));
   }
 }
 
 void gemm_small(SmallElem e, const SmallPlan& plan, const difflet_gemm_problem& q, int64_t n,
-                int64_t k, bool gate, int64_t rows_per_batch, void* scratch, hipStream_t s) {
+                int64_t k, bool gate, int64_t rows_per_batch, void* scratch, hipStream_t s,
+                const LoraDev* lora) {
   SmallArgs a = {};
   a.a = (const uint8_t*)q.a;
   a.w = (const uint8_t*)q.w;
@@ -533,6 +603,13 @@ void gemm_small(SmallElem e, const SmallPlan& plan, const difflet_gemm_problem& 
   }
   auto go = [&](auto et) {
     constexpr SmallElem E = decltype(et)::value;
+    if (lora) {
+      SmallLoraArgs la = {};
+      static_cast<SmallArgs&>(la) = a;
+      la.lora = *lora;
+      launch_small<E, false, true>(la, plan, s);
+      return;
+    }
     if (gate) launch_small<E, true>(a, plan, s);
     else launch_small<E, false>(a, plan, s);
   };

@@ -18,9 +18,17 @@ SmallPlan small_plan(SmallElem e, int64_t m, int64_t n, int64_t k, int cus, int6
                      double big_us);
 
 // Runs the plan: operands checked by the caller as for gemm.hip (F32: gemm_f32.hip, C, bias and
-// residual fp32, residual + (acc + bias)). gate: EPI_GATE_RESIDUAL.
+// residual fp32, residual + (acc + bias)). gate: EPI_GATE_RESIDUAL. lora: adapters of packed
+// requests (not with gate or F32).
+struct LoraDev;
 void gemm_small(SmallElem e, const SmallPlan& plan, const difflet_gemm_problem& q, int64_t n,
-                int64_t k, bool gate, int64_t rows_per_batch, void* scratch, hipStream_t s);
+                int64_t k, bool gate, int64_t rows_per_batch, void* scratch, hipStream_t s,
+                const LoraDev* lora = nullptr);
+
+// One problem without an epilogue, with adapters (gemm.hip); kind as difflet_rocm_gemm_single's,
+// the workspace this launch's alone.
+int gemm_lora(int kind, const difflet_gemm_problem& q, int64_t n, int64_t k, void* workspace,
+              int64_t workspace_bytes, hipStream_t stream, const LoraDev& lora);
 
 // Compute units of the current device (gemm.hip).
 int gemm_device_cus();

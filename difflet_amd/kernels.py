@@ -1389,3 +1389,80 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
             _row_head(q), _row_head(k), _row_head(v), _row_head(o), _ptr(q_starts), _ptr(k_starts),
             n, float(scale), int(out is None), _ptr(ws), nbytes, _stream(dev)), "packed_attention")
     return o
+
+
+def lora_linear(kind: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None,
+                down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor, starts: torch.Tensor,
+                ids: torch.Tensor, *, w_scale: torch.Tensor | None = None,
+                prepared: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """bf16 [M, N] = x W^T + bias + scale[a] (x down[a]^T) up[a]^T for bf16 x [M, K], a = ids[i] of
+    the request i with starts[i] <= row < starts[i + 1]; ids outside the adapters (-1) and rows of
+    no request have none. kind and w, w_scale as gemm_call's (K and N its multiples); down bf16
+    [adapters, rank, <= K], up bf16 [adapters, <= N, rank], scale fp32 [adapters], starts and ids
+    int32 on the device. prepared: x's codes and scales for the fp8 kinds, quantized here without."""
+    dev = _on_gpu(x, w, bias, down, up, scale, starts, ids, w_scale)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"lora_linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not chain")
+    m, k = x.shape
+    n = w.shape[0]
+    if x.dtype != torch.bfloat16 or down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16:
+        raise TypeError(f"lora_linear: x, down and up must be bf16, got {x.dtype}, {down.dtype}, "
+                        f"{up.dtype}")
+    if down.dim() != 3 or up.dim() != 3 or up.shape[0] != down.shape[0] or \
+            up.shape[2] != down.shape[1] or not 0 < down.shape[2] <= k or not 0 < up.shape[1] <= n:
+        raise ValueError(f"lora_linear: down [adapters, rank, {k}] and up [adapters, {n}, rank], got "
+                         f"{tuple(down.shape)} and {tuple(up.shape)}")
+    adapters, rank, kd = down.shape
+    if rank == 0 or kd % 8:
+        raise ValueError(f"lora_linear: rank {rank} and width {kd} of down (a multiple of 8)")
+    if scale.dtype != torch.float32 or scale.shape != (adapters,):
+        raise ValueError(f"lora_linear: scale must be fp32 [{adapters}], got {scale.dtype} "
+                         f"{tuple(scale.shape)}")
+    requests = _starts(starts, None, "lora_linear: starts")
+    if ids.dtype != torch.int32 or ids.shape != (requests,):
+        raise ValueError(f"lora_linear: ids must be int32 [{requests}], got {ids.dtype} "
+                         f"{tuple(ids.shape)}")
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.shape != (n,):
+            raise ValueError(f"lora_linear: bias must be bf16 [{n}], got {bias.dtype} "
+                             f"{tuple(bias.shape)}")
+        if bias.stride(0) != 1 or bias.data_ptr() % 8:
+            bias = bias.clone(memory_format=torch.contiguous_format)
+    y = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+    if m == 0:
+        return y
+
+    def aligned(t):  # the adapters' stacks, 16 bytes, in one piece
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+
+    down, up, scale, ids = aligned(down), aligned(up), scale.contiguous(), ids.contiguous()
+    x, w = _rows16(x, "lora_linear"), _rows2d(w, "lora_linear")
+    if x.stride(0) > _NEAR or w.stride(0) > _NEAR:
+        x, w = _near_rows(x), _near_rows(w)
+    kid = _KIND_ID[kind]
+    a, a_scale = x, None
+    with _current(dev):
+        if kid:
+            if prepared is not None:
+                a, a_scale = prepared
+            else:
+                a, a_scale = (quantize_mxfp8(x, swizzled=True) if kind == "mx"
+                              else quantize_fp8_rowwise(x))
+            _check_epilogue_operands(Problem(a, w, y, None, a_scale=a_scale, w_scale=w_scale), 0,
+                                     kind, n, k, _lib.EPI_NONE)
+            if a.shape != (m, k) or a.stride(1) != 1 or a.dtype not in _GEMM_A_DTYPES[kind] or \
+                    w.dtype not in _GEMM_A_DTYPES[kind]:
+                raise ValueError(f"lora_linear: {kind} weights are e4m3 codes, prepared e4m3 codes "
+                                 f"[{m}, {k}]")
+            _on_gpu(x, a, a_scale, w_scale)
+        elif w.dtype != torch.bfloat16:
+            raise TypeError(f"lora_linear: bf16 weights, got {w.dtype}")
+        nbytes = lib().difflet_rocm_lora_workspace_bytes(kid, m, n, k, rank, requests)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+        check(lib().difflet_rocm_lora_linear(
+            kid, _ptr(a), a.stride(0), _ptr(a_scale), _ptr(w), w.stride(0), _ptr(w_scale),
+            _ptr(bias), _ptr(y), n, m, n, k, _ptr(x), x.stride(0), kd, _ptr(down), _ptr(up),
+            up.shape[1], _ptr(scale), adapters, rank, _ptr(starts), _ptr(ids), requests, _ptr(ws),
+            ws.numel(), _stream(dev)), "lora_linear")
+    return y

@@ -643,6 +643,27 @@ int difflet_rocm_packed_attention(const void* q, const void* k, const void* v, v
                                   int zero_rest, void* workspace, int64_t workspace_bytes,
                                   difflet_stream_t stream);
 
+/* Low-rank adapters of packed requests beside a shared linear:
+ *   c[m] = x[m] W^T + bias + scale[a] (x[m] down[a]^T) up[a]^T, a = ids[i] of row m's request i;
+ * ids outside [0, adapters) (-1) and rows of no request have none. kind, a, lda, a_scale, w, ldw,
+ * w_scale, bias, c, ldc, n, k: as difflet_rocm_gemm_single's (a is x itself for kind 0, its codes
+ * otherwise). x: bf16 [m][x_cols] of row stride ldx, the rows the adapters read; down bf16
+ * [adapters][rank][x_cols], up bf16 [adapters][up_rows][rank], scale fp32 [adapters], contiguous;
+ * x_cols <= k a multiple of 8, up_rows <= n (columns past them have no adapter), rank <= 1024. The
+ * rank values x down^T are summed in fp32 and rounded to bf16 once, the result is rounded once. A
+ * column n whose up[a][n] holds an infinity or NaN is NaN in the rows of adapter a, and only there.
+ * workspace: this call's alone, 256-byte aligned, any contents, of difflet_rocm_lora_workspace_bytes
+ * (without the GEMM's share of it that runs whole tiles). */
+int64_t difflet_rocm_lora_workspace_bytes(int kind, int64_t m, int64_t n, int64_t k, int64_t rank,
+                                          int64_t requests);
+int difflet_rocm_lora_linear(int kind, const void* a, int64_t lda, const void* a_scale,
+                             const void* w, int64_t ldw, const void* w_scale, const void* bias,
+                             void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, const void* x,
+                             int64_t ldx, int64_t x_cols, const void* down, const void* up,
+                             int64_t up_rows, const float* scale, int64_t adapters, int64_t rank,
+                             const int32_t* starts, const int32_t* ids, int64_t requests,
+                             void* workspace, int64_t workspace_bytes, difflet_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,3 +114,40 @@ def test_packed_attention_entry_point_refusals():
     size = lib.difflet_rocm_packed_attention_workspace_bytes
     assert size(16, 32000, 16, 4, 7, 128) > 0  # single tokens: keys in pieces
     assert size(40000, 738, 2, 40, 1, 128) == 0 and size(0, 1, 1, 1, 1, 64) == 0
+
+
+def test_lora_linear_refusals():
+    from difflet_amd import kernels
+    from difflet_amd.backends.rocm.ops_impl.linear import lora_linear as f
+
+    x, w = torch.zeros(4, 64, dtype=BF16), torch.zeros(8, 64, dtype=BF16)
+    down, up = torch.zeros(1, 4, 64, dtype=BF16), torch.zeros(1, 8, 4, dtype=BF16)
+    one, s = torch.ones(1), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="device"):
+        f(x, w, None, down, up, one, s, s[:1])
+    with pytest.raises(ValueError, match="device"):
+        kernels.lora_linear("bf16", x, w, None, down, up, one, s, s[:1])
+
+
+def _lora(lib, **kw):
+    a = dict(kind=0, a=16, lda=64, a_scale=None, w=16, ldw=64, w_scale=None, bias=None, c=16, ldc=8,
+             m=1, n=8, k=64, x=16, ldx=64, x_cols=64, down=16, up=16, up_rows=8, scale=16, adapters=1,
+             rank=4, starts=16, ids=16, requests=1, ws=256, wb=1 << 20)
+    a.update(kw)
+    return lib.difflet_rocm_lora_linear(*a.values(), None)
+
+
+def test_lora_entry_point_refusals():
+    from difflet_amd import _lib
+
+    lib = _lib.load()
+    assert _lora(lib, m=0) == _lib.OK
+    for bad in (dict(kind=3), dict(m=-1), dict(n=0), dict(rank=0), dict(x_cols=72), dict(x_cols=60),
+                dict(x_cols=0), dict(up_rows=9), dict(up_rows=0), dict(x=None), dict(starts=None),
+                dict(ids=None), dict(down=None), dict(up=None), dict(scale=None), dict(ldx=56),
+                dict(x=8), dict(down=8), dict(ws=None), dict(wb=16), dict(ws=128),
+                dict(adapters=-1), dict(requests=-1)):
+        assert _lora(lib, **bad) == _lib.EINVAL, bad
+    assert _lora(lib, rank=1025) == _lib.EUNSUPPORTED
+    assert lib.difflet_rocm_lora_workspace_bytes(0, 0, 8, 64, 4, 1) == 0
+    assert lib.difflet_rocm_lora_workspace_bytes(5, 1, 8, 64, 4, 1) == 0
