@@ -4,10 +4,14 @@
 // GEMM adds v B_a^T in its accumulators (adapters.hpp). What the adapters cannot do without is one
 // more read of x, A and B; the GEMM's matrix work grows by rank / K.
 //
-// A workgroup takes 32 rows of one request and a part of K, its four wavefronts each every fourth
-// 64-wide step of it (MFMA 32x32x16, A first: a lane holds one row of x); x and A go from memory to
-// the matrix cores without LDS, since each is used once here. The wavefronts' sums meet in LDS.
-// Few rows: K is cut into `pieces` whose sums the GEMM adds in order.
+// Few rows: a workgroup takes 32 rows of one request and a part of K, its four wavefronts each every
+// fourth 64-wide step of it (MFMA 32x32x16, A first: a lane holds one row of x); x and A go from
+// memory to the matrix cores without LDS, since each is used once there, and the wavefronts' sums
+// meet in LDS. Many rows: a workgroup takes 128 rows, its wavefronts 32 each beside the same ranks,
+// and both operands come through a ring of LDS stages, 128 bytes of a row at a time: read straight
+// from memory, 32 rows at strides of the width share four sets of the L1, and each line is fetched
+// for every 32 bytes of it (34125 x 5120, rank 64: DOWN_A us; DOWN_B through LDS).
+// Where that leaves compute units idle, K is cut into `pieces` whose sums the GEMM adds in order.
 #include <algorithm>
 
 #include "adapters.hpp"
@@ -100,12 +104,108 @@ __global__ __launch_bounds__(256) void lora_down_kernel(const LoraDownArgs a) {
   }
 }
 
+constexpr int LORA_ROWS = 128;  // rows of a wide tile
+
+// The same for 128 rows of a request: 32 NR ranks, stages of 64 K elements (128 bytes a row) in a
+// ring of NS slots, NS - 1 of them in flight. Rows of x past the request, ranks past the adapter's
+// and K past the width read zero.
+template <int NR, int NS>
+__global__ __launch_bounds__(256, 1) void lora_down_wide_kernel(const LoraDownArgs a) {
+  constexpr int ROWS = LORA_ROWS + 32 * NR, SLOT = ROWS * 128, LPW = ROWS / 8 / 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NS * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, g = lane >> 5;
+  int id = blockIdx.x;
+  const int item = id % a.items;
+  id /= a.items;
+  const int piece = id % a.pieces, rb = id / a.pieces;
+  const PackedItem it = packed_item(a.starts, a.requests, a.m, 1, LORA_ROWS, false, item);
+  if (it.req < 0) return;
+  const int ad = a.ids[it.req];
+  if ((uint32_t)ad >= (uint32_t)a.adapters) return;
+  const int steps = (a.k + 63) / 64, per = (steps + a.pieces - 1) / a.pieces;
+  const int sbeg = piece * per, n = min(sbeg + per, steps) - sbeg;
+  const int rows = min(it.rows - it.tile * LORA_ROWS, LORA_ROWS);
+  const int ranks = min(a.rank - rb * 32 * NR, 32 * NR);
+  const int row0 = it.row0 + it.tile * LORA_ROWS;
+  constexpr uint32_t kOut = 0xfffffff0u;
+  const i32x4 rx = rsrc_of(a.x + (int64_t)row0 * a.ldx, (rows - 1) * a.ldx * 2 + (int64_t)a.k * 2);
+  const i32x4 rd = rsrc_of(a.down + ((int64_t)ad * a.rank + rb * 32 * NR) * a.k, (int64_t)ranks * a.k * 2);
+  // this wave's 1 KB loads of a stage: 8 rows of 8 chunks each, x's rows first
+  uint32_t off[LPW];
+  const int ch = lane & 7;
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int r = (wave * LPW + i) * 8 + (lane >> 3), kc = (ch ^ swz8s(r)) * 8;
+    const bool is_x = r < LORA_ROWS;
+    const int64_t o = is_x ? r * a.ldx * 2 : (int64_t)(r - LORA_ROWS) * a.k * 2;
+    off[i] = (is_x ? r < rows : r - LORA_ROWS < ranks) ? (uint32_t)o + kc * 2 : kOut;
+  }
+  auto issue = [&](int s) {
+    uint8_t* d = lds + (s % NS) * SLOT;
+    const int k0 = (sbeg + s) * 64;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int r = (wave * LPW + i) * 8 + (lane >> 3);
+      const bool in = s < n && k0 + (ch ^ swz8s(r)) * 8 < a.k && off[i] != kOut;
+      const uint32_t o = in ? off[i] + (uint32_t)k0 * 2 : kOut;
+      dma16s((wave * LPW + i) * 8 < LORA_ROWS ? rx : rd, d + (wave * LPW + i) * 1024, o, 0);
+    }
+  };
+  f32x16 acc[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) acc[i] = f32x16{};
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s) issue(s);
+  for (int s = 0; s < n; ++s) {
+    // this wave's loads of stage s have landed (NS - 2 younger stages may be in flight), its reads of
+    // stage s - 1 are done: the barrier publishes the one and frees the other's slot
+    wait_vm<(NS - 2) * LPW>();
+    asm volatile("s_barrier" ::: "memory");
+    issue(s + NS - 1);
+    const uint8_t* st = lds + (s % NS) * SLOT;
+    auto frag = [&](int r, int c) {
+      return *reinterpret_cast<const bf16x8*>(st + r * 128 + (((2 * c + g) ^ swz8s(r)) << 4));
+    };
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bf16x8 xv = frag(wave * 32 + col, c);
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(LORA_ROWS + i * 32 + col, c), xv,
+                                                         acc[i], 0, 0, 0);
+    }
+  }
+  wait_vm<0>();  // no load may outlive the workgroup's LDS
+  const float scale = a.scale[ad];
+  if (wave * 32 + col >= rows) return;
+  float* v = a.v + piece * a.v_piece + (int64_t)(row0 + wave * 32 + col) * a.ldv;
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = (rb * NR + i) * 32 + 8 * q + 4 * g;
+      if (r >= a.ldv) continue;
+      f32x4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = r + e < a.rank ? acc[i][4 * q + e] * scale : 0.f;
+      *reinterpret_cast<f32x4*>(v + r) = t;
+    }
+}
+
 static int64_t lora_ldv(int64_t rank) { return (rank + 7) / 8 * 8; }
-static int64_t lora_items(int64_t m, int64_t requests) { return (m + 31) / 32 + requests; }
-// K pieces: workgroups for every compute unit twice over, a 64-wide step for each wavefront
+// Rows from which the wide tiles run: below, their workgroups are too few to draw x's bytes.
+static bool lora_wide(int64_t m, int64_t requests) { return m >= 2048 && m >= 32 * requests; }
+static int64_t lora_items(int64_t m, int64_t requests) {
+  const int64_t rows = lora_wide(m, requests) ? LORA_ROWS : 32;
+  return (m + rows - 1) / rows + requests;
+}
+// K pieces: a workgroup for every compute unit, twice over for the small tiles, and at least 4
+// stages (a 64-wide step for each wavefront) a piece
 static int64_t lora_pieces(int64_t m, int64_t k, int64_t requests) {
-  const int64_t steps = (k + 63) / 64;
-  return std::max<int64_t>(1, std::min<int64_t>({512 / lora_items(m, requests), steps / 4, 16}));
+  const int64_t steps = (k + 63) / 64, want = lora_wide(m, requests) ? 256 : 512;
+  return std::max<int64_t>(1, std::min<int64_t>({want / lora_items(m, requests), steps / 4, 16}));
 }
 static int64_t lora_v_bytes(int64_t m, int64_t k, int64_t rank, int64_t requests) {
   return (lora_pieces(m, k, requests) * m * lora_ldv(rank) * 4 + 255) / 256 * 256;
@@ -146,6 +246,8 @@ extern "C" int difflet_rocm_lora_linear(int kind, const void* a, int64_t lda, co
   if (m == 0) return DIFFLET_OK;
   DLT_REQUIRE(x && starts && (requests == 0 || ids) && (adapters == 0 || (down && up && scale)),
               DIFFLET_EINVAL, "%s: null pointer", name);
+  DLT_REQUIRE(ldx <= (1LL << 23) || m < 2, DIFFLET_EUNSUPPORTED, "%s: rows of x more than 16 MB apart",
+              name);
   DLT_REQUIRE(ldx >= x_cols && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)down | (uintptr_t)up) & 15) == 0,
               DIFFLET_EINVAL, "%s: rows of x and the adapters must start on 16 bytes", name);
   const int64_t vb = lora_v_bytes(m, x_cols, rank, requests);
@@ -165,9 +267,17 @@ extern "C" int difflet_rocm_lora_linear(int kind, const void* a, int64_t lda, co
     const int64_t grid = (int64_t)d.items * d.pieces * d.blocks;
     DLT_REQUIRE(grid < (1LL << 31), DIFFLET_EUNSUPPORTED, "%s: too many tiles", name);
     const dim3 g((unsigned)grid), b(256);
-    if (nr == 1) hipLaunchKernelGGL((lora_down_kernel<1>), g, b, 0, s, d);
-    else if (nr == 2) hipLaunchKernelGGL((lora_down_kernel<2>), g, b, 0, s, d);
-    else hipLaunchKernelGGL((lora_down_kernel<4>), g, b, 0, s, d);
+    if (lora_wide(m, requests)) {
+      if (nr == 1) hipLaunchKernelGGL((lora_down_wide_kernel<1, 4>), g, b, 0, s, d);
+      else if (nr == 2) hipLaunchKernelGGL((lora_down_wide_kernel<2, 4>), g, b, 0, s, d);
+      else hipLaunchKernelGGL((lora_down_wide_kernel<4, 4>), g, b, 0, s, d);
+    } else if (nr == 1) {
+      hipLaunchKernelGGL((lora_down_kernel<1>), g, b, 0, s, d);
+    } else if (nr == 2) {
+      hipLaunchKernelGGL((lora_down_kernel<2>), g, b, 0, s, d);
+    } else {
+      hipLaunchKernelGGL((lora_down_kernel<4>), g, b, 0, s, d);
+    }
     const int st = dlt_check_launch(name);
     if (st != DIFFLET_OK) return st;
   } else {

@@ -1,9 +1,33 @@
-// The small-launch GEMM (gemm_small.hip) as gemm.hip's dispatch sees it.
+// The small-launch GEMM (gemm_small.hip) as gemm.hip's dispatch sees it, and the direct-to-LDS loads
+// that it shares with adapters.hip.
 #pragma once
 
 #include "common.hpp"
 
 namespace dlt {
+
+// direct-to-LDS load of 16 bytes per lane (as attention.hip's dma16, with a scalar offset):
+// untracked by the compiler, waited for by the K loop's own vmcnt
+typedef __attribute__((address_space(3))) void lds_void_t;
+__device__ __forceinline__ void dma16s(i32x4 r, const uint8_t* lds_ptr, uint32_t voff,
+                                       uint32_t soff) {
+  const uint32_t la = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_t*)lds_ptr);
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(la), "v"(voff), "s"(r), "s"(soff)
+               : "memory", "m0");
+}
+__device__ __forceinline__ i32x4 rsrc_of(const void* base, int64_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const uint32_t n = bytes > 0xffffffffLL ? 0xffffffffu : (uint32_t)bytes;
+  return i32x4{(int)(uint32_t)a, (int)(uint32_t)((a >> 32) & 0xffffu), (int)n, 0x00020000};
+}
+template <int VM>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(VM >= 0 && VM < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (VM & 15) | ((VM >> 4) << 14));  // and lgkmcnt(0)
+}
+__device__ __forceinline__ int swz8s(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 enum class SmallElem { BF16, FP8, MX, F32 };
 

@@ -4,16 +4,22 @@
 // pass over the keys. The query heads of a key head are extra rows: row r of a request's r-space
 // is token r / group, head r % group, so a tile reads its keys once for all of them.
 //
-// A workgroup takes a tile of 128 such rows (four wavefronts of 32) of one request and key head
-// and finds them itself from the row numbers on the device: the host knows only bounds, and a
-// captured graph follows new lengths. Scores are computed transposed (S^T = K Q^T, 32x32x16), so
-// the statistics of a row live in two lanes and P feeds the second product from registers, as in
-// attention.hip. Keys come in tiles of 64 through two LDS buffers, K row-major, V transposed while
-// it is written. Buffer ranges end with the request's last key: rows of the next request or past
-// the tensor read as zero, whatever lies there.
+// A workgroup finds its tile of such rows (of one request and key head) itself, from the row numbers
+// on the device: the host knows only bounds, and a captured graph follows new lengths. Scores are
+// computed transposed (S^T = K Q^T, 32x32x16), so the statistics of a row live in two lanes and P
+// feeds the second product from registers, as in attention.hip. Buffer ranges end with the
+// request's last key: rows of the next request or past the tensor read as zero, whatever lies there.
 //
-// Few tiles (single tokens, short prompts): a request's keys are cut into `pieces`, each with
-// statistics of its own, joined by a second kernel in the order of the pieces.
+// packed_attn_kernel: 128 rows (four wavefronts of 32), tiles of 64 keys through two LDS buffers, K
+// row-major, V transposed while it is written.
+// packed_attn_few_kernel: few rows a request (single tokens): 32 rows, whose four wavefronts take 32
+// keys each of tiles of 128 and join what they have in LDS.
+//
+// Few tiles: the launch has a fixed number of workgroups, which cut the requests' keys into chunks of
+// about one length, one or two a workgroup (the length follows from the row numbers on the
+// device). A row tile of several chunks leaves the unnormalized sums of each and their statistics in
+// the workspace, joined by packed_attn_join in the order of the chunks. 16 single tokens over 0 to
+// 8000 states (4 key heads): 28 + 6 us with every request's keys in 12 pieces, CHUNK_A us so.
 #include <float.h>
 
 #include <algorithm>
@@ -32,260 +38,514 @@ struct PackedAttnArgs {
   const int32_t* q_starts;
   const int32_t* k_starts;
   int requests, rows_q, rows_k, kv_heads, group;
-  int items;       // tiles per key head, at most
-  int pieces;      // of a request's keys
-  int zero_rest;   // rows of no request come out zero (else are not written)
+  int items;         // row tiles per key head, at most
+  int zero_rest;     // rows of no request come out zero (else are not written)
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // 0x80008000 for a negative scale
-  float* part;       // [pieces][rows_q][heads][D] unnormalized sums (pieces > 1)
-  f32x2* stats;      // [pieces][rows_q][heads]: running maximum (scaled), sum
+  int groups;           // workgroups of a launch that cuts keys into chunks (0: whole keys)
+  int slots;            // of the workspace: row numbers out of order could ask for more
+  float* part;          // [slots][block][D] unnormalized sums, slot = item
+  f32x2* stats;         // [slots][block]: running maximum (scaled), sum; sum -1: a chunk without keys
 };
 
-constexpr int PA_ROWS = 128, PA_KEYS = 64;
-constexpr int PA_VT = PA_KEYS * 2 + 16;  // bytes per V^T row
+// ------------------------------------------------------------------ the schedule
+// A row tile, its request's keys and the chunk of them that runs here. Items count chunks within
+// row tiles within requests; an item of key head h is workgroup item `item * kv_heads + h`.
+struct PackedWork {
+  PackedItem it;
+  int kbeg, keys;           // the request's keys
+  int chunk, chunks, first; // of the row tile; item of its chunk 0
+};
 
-template <typename T, int D, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void packed_attn_kernel(const PackedAttnArgs a) {
-  typedef typename MfmaT<T>::frag frag;
-  constexpr int KP = D * 2 + 16, NC = D / 16, NDT = D / 32, KCH = D / 8;
-  __shared__ __attribute__((aligned(16))) uint8_t sk[2][PA_KEYS * KP];
-  __shared__ __attribute__((aligned(16))) uint8_t sv[2][D * PA_VT];
-  auto kofs = [](int row, int chunk) { return row * KP + (chunk << 4); };
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int col = lane & 31, g = lane >> 5;
-
-  // ids go round the 8 XCDs: each takes a run of (key head, tile), the tiles of a head side by
-  // side, so a request's keys stay in one L2
-  int id = blockIdx.x;
-  if ((gridDim.x & 7) == 0) id = (id & 7) * (gridDim.x >> 3) + (id >> 3);
-  const int item = id % a.items;
-  const int hp = id / a.items;
-  const int piece = SPLIT ? hp % a.pieces : 0;
-  const int hk = SPLIT ? hp / a.pieces : hp;
-  const PackedItem it = packed_item(a.q_starts, a.requests, a.rows_q, a.group, PA_ROWS,
-                                    a.zero_rest != 0, item);
-  if (it.req < 0) return;
-  int kbeg = 0, keys = 0;
-  if (it.req < a.requests) {
-    kbeg = packed_start(a.k_starts, it.req, a.rows_k);
-    keys = max(packed_start(a.k_starts, it.req + 1, a.rows_k) - kbeg, 0);
+__device__ __forceinline__ void packed_keys(const PackedAttnArgs& a, int i, int& kbeg, int& keys) {
+  kbeg = 0, keys = 0;
+  if (i < a.requests) {
+    kbeg = packed_start(a.k_starts, i, a.rows_k);
+    keys = max(packed_start(a.k_starts, i + 1, a.rows_k) - kbeg, 0);
   }
-  int j_beg = 0, j_end = keys;
-  if (SPLIT) {
-    const int tiles = (keys + PA_KEYS - 1) / PA_KEYS, per = (tiles + a.pieces - 1) / a.pieces;
-    j_beg = min(piece * per * PA_KEYS, keys);
-    j_end = min(j_beg + per * PA_KEYS, keys);
+}
+
+// The chunks of a launch of at most PACKED_LANES requests, one request a lane: loaded once, every
+// item of a workgroup is then found by a ballot.
+constexpr int PACKED_LANES = kWave - 2;
+template <int BLOCK, int KEYT> struct PackedChunks {
+  int r0, len, kbeg, keys;  // the lane's request (or rows of none)
+  int tiles, chunks, upto;  // row tiles, chunks of each; items up to and with the lane's
+  __device__ __forceinline__ void scan(const PackedAttnArgs& a) {
+    const int i = threadIdx.x & (kWave - 1);
+    packed_rows(a.q_starts, a.requests, a.rows_q, a.zero_rest != 0, i, r0, len);
+    packed_keys(a, i, kbeg, keys);
+    tiles = (len * a.group + BLOCK - 1) / BLOCK;
+    const int kt = (keys + KEYT - 1) / KEYT;
+    // key tiles per chunk, so that the chunks of all heads, a last short one for every row tile among
+    // them, are one a workgroup (a schedule: every wavefront rounds alike, and that is all it takes)
+    const float work = wave_sum((float)tiles * (float)kt) * (float)a.kv_heads;
+    const float spare = (float)a.groups - wave_sum((float)tiles) * (float)a.kv_heads;
+    const int per = max(1, (int)ceilf(work / fmaxf(spare, 0.25f * (float)a.groups)));
+    chunks = max(1, (kt + per - 1) / per);
+    upto = wave_prefix(tiles * chunks);
   }
+  // the row tiles of lane l's request
+  __device__ __forceinline__ PackedWork work_of(const PackedAttnArgs& a, int l) const {
+    PackedWork w;
+    w.it.req = min(l, a.requests);
+    w.it.tile = w.chunk = 0;
+    w.it.row0 = __builtin_amdgcn_readlane(r0, l);
+    w.it.rows = __builtin_amdgcn_readlane(len, l);
+    w.kbeg = __builtin_amdgcn_readlane(kbeg, l);
+    w.keys = __builtin_amdgcn_readlane(keys, l);
+    w.chunks = __builtin_amdgcn_readlane(chunks, l);
+    w.first = __builtin_amdgcn_readlane(upto - tiles * chunks, l);
+    return w;
+  }
+  __device__ __forceinline__ PackedWork item(const PackedAttnArgs& a, int n) const {
+    const uint64_t past = __ballot(upto > n);
+    if (!past) {
+      PackedWork w = {};
+      w.it.req = -1;
+      return w;
+    }
+    PackedWork w = work_of(a, __ffsll((unsigned long long)past) - 1);
+    w.it.tile = (n - w.first) / w.chunks;
+    w.chunk = (n - w.first) % w.chunks;
+    return w;
+  }
+};
 
-  // this lane's row of the request
-  const int r = it.tile * PA_ROWS + wave * 32 + col;
-  const int tok = r / a.group, head = hk * a.group + (r - tok * a.group);
-  const bool there = (uint32_t)tok < (uint32_t)it.rows;
-  const int64_t row = it.row0 + tok;
+// SPLIT: item `item` of the chunks, else of the row tiles, each with all of its keys.
+template <bool SPLIT, typename Chunks>
+__device__ __forceinline__ PackedWork packed_work(const PackedAttnArgs& a, const Chunks& chunks,
+                                                  int block, int item) {
+  if constexpr (SPLIT) return chunks.item(a, item);
+  PackedWork w = {};
+  w.it = packed_item(a.q_starts, a.requests, a.rows_q, a.group, block, a.zero_rest != 0, item);
+  w.chunks = 1;
+  if (w.it.req >= 0) packed_keys(a, w.it.req, w.kbeg, w.keys);
+  return w;
+}
 
-  frag qf[NC];
+// Keys [j_beg, j_end) of the request that chunk `chunk` of `chunks` covers.
+__device__ __forceinline__ void packed_range(const PackedWork& w, int key_tile, int& j_beg,
+                                             int& j_end) {
+  const int cut = ((w.keys + key_tile - 1) / key_tile + w.chunks - 1) / w.chunks * key_tile;
+  j_beg = min(w.chunk * cut, w.keys);
+  j_end = min(j_beg + cut, w.keys);
+}
+
+// ------------------------------------------------------------------ pieces of a tile
+// Q fragments of a lane: its row, channels 16 c + 8 g .. + 8.
+template <typename T, int D>
+__device__ __forceinline__ void packed_load_q(const PackedAttnArgs& a, bool there, int64_t row,
+                                              int head, int g, typename MfmaT<T>::frag (&qf)[D / 16]) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
+  for (int c = 0; c < D / 16; ++c) {
     u32x4 raw = {0u, 0u, 0u, 0u};
     if (there)
       raw = *reinterpret_cast<const u32x4*>(a.q + (row * a.qs[0] + head * a.qs[1] + c * 16 + g * 8) * 2);
 #pragma unroll
     for (int e = 0; e < 4; ++e) raw[e] ^= a.q_sign;
-    qf[c] = __builtin_bit_cast(frag, raw);
+    qf[c] = __builtin_bit_cast(typename MfmaT<T>::frag, raw);
   }
+}
 
-  const uint8_t* kp = a.k + ((int64_t)kbeg * a.ks[0] + hk * a.ks[1]) * 2;
-  const uint8_t* vp = a.v + ((int64_t)kbeg * a.vs[0] + hk * a.vs[1]) * 2;
-  const int64_t krow = a.ks[0] * 2, vrow = a.vs[0] * 2;
-  constexpr int KRI = 256 / KCH, NKI = PA_KEYS / KRI;  // K rows per pass, passes
-  const int kr = tid / KCH, kc = tid % KCH;
-  const int vkg = tid & 15, vdg = tid >> 4;
-  const bool v_on = vdg < D / 8;
-  const int vt_pos = vt_quad_pos(vkg) * 8;
-  u32x4 gk[NKI], gv[4];
-  auto load_tile = [&](int j0) {  // the range ends with the last key's channels
-    const int n = min(j_end - j0, PA_KEYS);
-    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kp + j0 * krow, (uint32_t)((n - 1) * krow + D * 2));
-    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vp + j0 * vrow, (uint32_t)((n - 1) * vrow + D * 2));
+// Keys and values of a tile of KEYS keys by 256 threads: from memory into registers (zero past the
+// n keys there are), from there into LDS, K rows of KP bytes, V^T rows of VT bytes with the key
+// quads of each 16 in vt_quad_pos's order.
+template <int D, int KEYS> struct PackedTile {
+  static constexpr int KP = D * 2 + 16, VT = KEYS * 2 + 16, KCH = D / 8;
+  static constexpr int KRI = 256 / KCH, NKI = KEYS / KRI;              // K rows per pass, passes
+  static constexpr int VQ = KEYS / 4, VDP = 256 / VQ;                  // key quads, channel groups
+  static constexpr int NVI = D / 8 > VDP ? D / 8 / VDP : 1;            // a pass; passes
+  u32x4 k[NKI], v[NVI][4];
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int64_t krow,
+                                       int64_t vrow, int n) {
+    const int tid = threadIdx.x;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kp, (uint32_t)((n - 1) * krow + D * 2));
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vp, (uint32_t)((n - 1) * vrow + D * 2));
+    constexpr uint32_t kOut = 0xfffffff0u;  // past every range
 #pragma unroll
     for (int i = 0; i < NKI; ++i) {
-      const int key = kr + KRI * i;
-      gk[i] = buf_load16(rk, key < n ? (uint32_t)(key * krow) + kc * 16 : 0xfffffff0u);
+      const int key = tid / KCH + KRI * i;
+      k[i] = buf_load16(rk, key < n ? (uint32_t)(key * krow) + (tid % KCH) * 16 : kOut);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = vkg * 4 + i;
-      gv[i] = v_on ? buf_load16(rv, key < n ? (uint32_t)(key * vrow) + vdg * 16 : 0xfffffff0u)
-                   : u32x4{0u, 0u, 0u, 0u};
-    }
-  };
-  auto store_tile = [&](int st) {
+    for (int p = 0; p < NVI; ++p)
 #pragma unroll
-    for (int i = 0; i < NKI; ++i) *reinterpret_cast<u32x4*>(&sk[st][kofs(kr + KRI * i, kc)]) = gk[i];
-    if (!v_on) return;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {  // the 4 keys' values of a channel side by side
-      const int w = d >> 1, sh = (d & 1) * 16;
-      const uint32_t k0 = (gv[0][w] >> sh) & 0xffffu, k1 = (gv[1][w] >> sh) & 0xffffu;
-      const uint32_t k2 = (gv[2][w] >> sh) & 0xffffu, k3 = (gv[3][w] >> sh) & 0xffffu;
-      *reinterpret_cast<u32x2*>(&sv[st][(vdg * 8 + d) * PA_VT + vt_pos]) =
-          u32x2{k0 | (k1 << 16), k2 | (k3 << 16)};
-    }
-  };
-
-  f32x16 acc[NDT];
-#pragma unroll
-  for (int i = 0; i < NDT; ++i) acc[i] = f32x16{};
-  float m_run = -INFINITY, l_run = 0.f;
-  if (j_beg < j_end) {
-    load_tile(j_beg);
-    store_tile(0);
+      for (int i = 0; i < 4; ++i) {
+        const int key = (tid % VQ) * 4 + i, dg = p * VDP + tid / VQ;
+        v[p][i] = buf_load16(rv, key < n && dg < D / 8 ? (uint32_t)(key * vrow) + dg * 16 : kOut);
+      }
   }
-  __syncthreads();
-  for (int j0 = j_beg, st = 0; j0 < j_end; j0 += PA_KEYS, st ^= 1) {
-    const bool more = j0 + PA_KEYS < j_end;
-    if (more) load_tile(j0 + PA_KEYS);
-    f32x16 s[2];
+  __device__ __forceinline__ void store(uint8_t* sk, uint8_t* sv) const {
+    const int tid = threadIdx.x;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < NKI; ++i)
+      *reinterpret_cast<u32x4*>(sk + (tid / KCH + KRI * i) * KP + (tid % KCH) * 16) = k[i];
+    const int pos = vt_quad_pos(tid % VQ) * 8;
+#pragma unroll
+    for (int p = 0; p < NVI; ++p) {
+      const int dg = p * VDP + tid / VQ;
+      if (dg >= D / 8) continue;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {  // the 4 keys' values of a channel side by side
+        const int w = d >> 1, sh = (d & 1) * 16;
+        const uint32_t k0 = (v[p][0][w] >> sh) & 0xffffu, k1 = (v[p][1][w] >> sh) & 0xffffu;
+        const uint32_t k2 = (v[p][2][w] >> sh) & 0xffffu, k3 = (v[p][3][w] >> sh) & 0xffffu;
+        *reinterpret_cast<u32x2*>(sv + (dg * 8 + d) * VT + pos) = u32x2{k0 | (k1 << 16), k2 | (k3 << 16)};
+      }
+    }
+  }
+};
+
+// Online softmax of a lane's row and the second product, over NT x 32 keys from key0 of LDS on.
+// Scores stay raw (p = exp2(s c - m), m in scaled units, c > 0); keys from `left` on do not exist.
+template <typename T, int D> struct PackedRow {
+  typedef typename MfmaT<T>::frag frag;
+  f32x16 acc[D / 32];
+  float m_run, l_run;
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
+    m_run = -INFINITY, l_run = 0.f;
+  }
+  template <int NT>
+  __device__ __forceinline__ void step(const frag (&qf)[D / 16], const uint8_t* sk, int kp,
+                                       const uint8_t* sv, int vt, int key0, int left, float c) {
+    const int lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    f32x16 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       s[t] = f32x16{};
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        s[t] = MfmaT<T>::mma(*reinterpret_cast<const frag*>(&sk[st][kofs(t * 32 + col, c * 2 + g)]),
-                             qf[c], s[t]);
+      for (int i = 0; i < D / 16; ++i)
+        s[t] = MfmaT<T>::mma(
+            *reinterpret_cast<const frag*>(sk + (key0 + t * 32 + col) * kp + (i * 2 + g) * 16), qf[i],
+            s[t]);
     }
-    if (j0 + PA_KEYS > j_end) {  // keys past the request's last do not exist
+    if (left < NT * 32) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          if (j0 + t * 32 + (v >> 2) * 8 + g * 4 + (v & 3) >= j_end) s[t][v] = -INFINITY;
+          if (t * 32 + (v >> 2) * 8 + g * 4 + (v & 3) >= left) s[t][v] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[t][v]);
     mx = pair_max(mx);
-    const float m_new = fmaxf(m_run, mx * a.scale_log2);
+    const float m_new = fmaxf(m_run, mx * c);
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
     m_run = m_new;
     float ls = 0.f;
-    uint32_t pp[2][8];
+    uint32_t pp[NT][8];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int v = 0; v < 16; v += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][v], a.scale_log2, -m_use));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][v + 1], a.scale_log2, -m_use));
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][v], c, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][v + 1], c, -m_use));
         ls += p0 + p1;
         pp[t][v >> 1] = MfmaT<T>::pack2(p0, p1);
       }
     l_run = l_run * alpha + ls;
     if (__any(alpha != 1.0f)) {
 #pragma unroll
-      for (int i = 0; i < NDT; ++i)
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[i][v] *= alpha;
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
+      for (int hh = 0; hh < 2; ++hh) {  // 16 keys: {4g .. 4g + 3, 8 + 4g .. 8 + 4g + 3}
         u32x4 pb;
 #pragma unroll
         for (int u = 0; u < 4; ++u) pb[u] = pp[t][hh * 4 + u];
         const frag pf = __builtin_bit_cast(frag, pb);
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
+        for (int dt = 0; dt < D / 32; ++dt)
           acc[dt] = MfmaT<T>::mma(*reinterpret_cast<const frag*>(
-                                      &sv[st][(dt * 32 + col) * PA_VT + (t * 32 + hh * 16 + g * 8) * 2]),
+                                      sv + (dt * 32 + col) * vt + (key0 + t * 32 + hh * 16 + g * 8) * 2),
                                   pf, acc[dt]);
       }
-    if (more) store_tile(st ^ 1);
-    __syncthreads();
   }
+};
 
-  // lane: its row, channels dt * 32 + (v / 4) * 8 + 4 g + v % 4
-  const float l = pair_sum(l_run);
-  if (!there) return;
-  if constexpr (SPLIT) {
-    const int64_t at = ((int64_t)piece * a.rows_q + row) * ((int64_t)a.kv_heads * a.group) + head;
-    if (g == 0) a.stats[at] = f32x2{m_run, j_beg < j_end ? l : -1.0f};
-    if (j_beg >= j_end) return;  // no keys: the join reads no sums there
-    float* p = a.part + at * D;
+// ------------------------------------------------------------------ kernels
+constexpr int PA_ROWS = 128, PA_KEYS = 64;
+
+template <typename T, int D, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void packed_attn_kernel(const PackedAttnArgs a) {
+  typedef PackedTile<D, PA_KEYS> Tile;
+  __shared__ __attribute__((aligned(16))) uint8_t sk[2][PA_KEYS * Tile::KP];
+  __shared__ __attribute__((aligned(16))) uint8_t sv[2][D * Tile::VT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 31, g = lane >> 5;
+  PackedChunks<PA_ROWS, PA_KEYS> chunks;
+  if (SPLIT) chunks.scan(a);
+  // whole keys: ids go round the 8 XCDs, and each takes a run of (key head, tile), the tiles of a head
+  // side by side, so that a request's keys stay in one L2
+  int id = blockIdx.x;
+  if (!SPLIT && (gridDim.x & 7) == 0) id = (id & 7) * (gridDim.x >> 3) + (id >> 3);
+  for (;; id += gridDim.x) {
+    const int hk = SPLIT ? id % a.kv_heads : id / a.items;
+    const PackedWork w = packed_work<SPLIT>(a, chunks, PA_ROWS, SPLIT ? id / a.kv_heads : id % a.items);
+    if (w.it.req < 0 || (SPLIT && id >= a.slots)) return;
+    int j_beg, j_end;
+    packed_range(w, PA_KEYS, j_beg, j_end);
+    const int r = w.it.tile * PA_ROWS + wave * 32 + col;  // this lane's row of the request
+    const int tok = r / a.group, head = hk * a.group + (r - tok * a.group);
+    const bool there = (uint32_t)tok < (uint32_t)w.it.rows;
+    const int64_t row = w.it.row0 + tok;
+    typename MfmaT<T>::frag qf[D / 16];
+    packed_load_q<T, D>(a, there, row, head, g, qf);
+    const uint8_t* kp = a.k + ((int64_t)w.kbeg * a.ks[0] + hk * a.ks[1]) * 2;
+    const uint8_t* vp = a.v + ((int64_t)w.kbeg * a.vs[0] + hk * a.vs[1]) * 2;
+    const int64_t krow = a.ks[0] * 2, vrow = a.vs[0] * 2;
+    Tile tile;
+    auto load = [&](int j0) {
+      tile.load(kp + j0 * krow, vp + j0 * vrow, krow, vrow, min(j_end - j0, PA_KEYS));
+    };
+    PackedRow<T, D> st;
+    st.reset();
+    if (j_beg < j_end) {
+      load(j_beg);
+      tile.store(sk[0], sv[0]);
+    }
+    __syncthreads();
+    for (int j0 = j_beg, b = 0; j0 < j_end; j0 += PA_KEYS, b ^= 1) {
+      const bool more = j0 + PA_KEYS < j_end;
+      if (more) load(j0 + PA_KEYS);
+      st.template step<2>(qf, sk[b], Tile::KP, sv[b], Tile::VT, 0, j_end - j0, a.scale_log2);
+      if (more) tile.store(sk[b ^ 1], sv[b ^ 1]);
+      __syncthreads();
+    }
+    // lane: its row, channels dt * 32 + (v / 4) * 8 + 4 g + v % 4
+    const float l = pair_sum(st.l_run);
+    if (SPLIT && w.chunks > 1) {
+      const int64_t at = (int64_t)id * PA_ROWS + wave * 32 + col;
+      if (there && g == 0) a.stats[at] = f32x2{st.m_run, j_beg < j_end ? l : -1.0f};
+      if (there && j_beg < j_end) {
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
+        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        *reinterpret_cast<f32x4*>(p + dt * 32 + u * 8 + g * 4) =
-            f32x4{acc[dt][4 * u], acc[dt][4 * u + 1], acc[dt][4 * u + 2], acc[dt][4 * u + 3]};
-  } else {
-    const float inv = keys == 0 ? 0.f : 1.0f / l;  // no keys: zeros
-    T* op = reinterpret_cast<T*>(a.o) + row * a.os[0] + head * a.os[1];
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<f32x4*>(a.part + at * D + dt * 32 + u * 8 + g * 4) =
+                f32x4{st.acc[dt][4 * u], st.acc[dt][4 * u + 1], st.acc[dt][4 * u + 2],
+                      st.acc[dt][4 * u + 3]};
+      }
+    } else if (there) {
+      const float inv = w.keys == 0 ? 0.f : 1.0f / l;  // no keys: zeros
+      T* op = reinterpret_cast<T*>(a.o) + row * a.os[0] + head * a.os[1];
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
+      for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        *reinterpret_cast<u32x2*>(op + dt * 32 + u * 8 + g * 4) =
-            u32x2{MfmaT<T>::pack2(acc[dt][4 * u] * inv, acc[dt][4 * u + 1] * inv),
-                  MfmaT<T>::pack2(acc[dt][4 * u + 2] * inv, acc[dt][4 * u + 3] * inv)};
+        for (int u = 0; u < 4; ++u)
+          *reinterpret_cast<u32x2*>(op + dt * 32 + u * 8 + g * 4) =
+              u32x2{MfmaT<T>::pack2(st.acc[dt][4 * u] * inv, st.acc[dt][4 * u + 1] * inv),
+                    MfmaT<T>::pack2(st.acc[dt][4 * u + 2] * inv, st.acc[dt][4 * u + 3] * inv)};
+    }
+    if (!SPLIT) return;
   }
 }
 
-// The pieces of a row joined: a wavefront per (row, head). A piece without keys has sum -1 and no
-// stored output; a row without any is zero. (A sum of 0, all scores -inf, gives NaN as it does
-// in one piece.)
-template <typename T, int D>
+// Tiles of 32 rows against tiles of 128 keys, 32 of them each wavefront's: with the few rows of
+// single tokens every wavefront's matrix work and softmax is on keys of its own, where
+// packed_attn_kernel's second to fourth would work on rows that are not there. The keys of the next
+// tile wait in registers while this one's are in LDS, so two workgroups fit a compute unit and keep
+// 128 KB of keys in flight on it.
+constexpr int PF_ROWS = 32, PF_KEYS = 128;
+
+template <typename T, int D, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void packed_attn_few_kernel(const PackedAttnArgs a) {
+  typedef PackedTile<D, PF_KEYS> Tile;
+  constexpr int JOIN = 4 * PF_ROWS * D * 4, TILES = PF_KEYS * Tile::KP + D * Tile::VT;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[TILES > JOIN ? TILES : JOIN];
+  __shared__ f32x2 ml[4][PF_ROWS];
+  uint8_t *sk = lds, *sv = lds + PF_KEYS * Tile::KP;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 31, g = lane >> 5;
+  PackedChunks<PF_ROWS, PF_KEYS> chunks;
+  if (SPLIT) chunks.scan(a);
+  int id = blockIdx.x;
+  if (!SPLIT && (gridDim.x & 7) == 0) id = (id & 7) * (gridDim.x >> 3) + (id >> 3);
+  for (;; id += gridDim.x) {
+    const int hk = SPLIT ? id % a.kv_heads : id / a.items;
+    const PackedWork w = packed_work<SPLIT>(a, chunks, PF_ROWS, SPLIT ? id / a.kv_heads : id % a.items);
+    if (w.it.req < 0 || (SPLIT && id >= a.slots)) return;
+    int j_beg, j_end;
+    packed_range(w, PF_KEYS, j_beg, j_end);
+    const uint8_t* kp = a.k + ((int64_t)w.kbeg * a.ks[0] + hk * a.ks[1]) * 2;
+    const uint8_t* vp = a.v + ((int64_t)w.kbeg * a.vs[0] + hk * a.vs[1]) * 2;
+    const int64_t krow = a.ks[0] * 2, vrow = a.vs[0] * 2;
+    Tile tile;
+    auto load = [&](int j0) {
+      tile.load(kp + j0 * krow, vp + j0 * vrow, krow, vrow, min(j_end - j0, PF_KEYS));
+    };
+    if (j_beg < j_end) load(j_beg);
+    const int r = w.it.tile * PF_ROWS + col;
+    const int tok = r / a.group, head = hk * a.group + (r - tok * a.group);
+    typename MfmaT<T>::frag qf[D / 16];
+    packed_load_q<T, D>(a, (uint32_t)tok < (uint32_t)w.it.rows, (int64_t)w.it.row0 + tok, head, g, qf);
+    PackedRow<T, D> st;
+    st.reset();
+    for (int j0 = j_beg; j0 < j_end; j0 += PF_KEYS) {
+      tile.store(sk, sv);
+      __syncthreads();
+      if (j0 + PF_KEYS < j_end) load(j0 + PF_KEYS);
+      st.template step<1>(qf, sk, Tile::KP, sv, Tile::VT, wave * 32, j_end - j0 - wave * 32,
+                          a.scale_log2);
+      __syncthreads();
+    }
+    // ---- the four wavefronts' parts of each row, in their order
+    const float l_w = pair_sum(st.l_run);
+    if (g == 0) ml[wave][col] = f32x2{st.m_run, l_w};
+    __syncthreads();
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i][col][0]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += ml[i][col][1] * __builtin_amdgcn_exp2f(ml[i][col][0] - m_use);
+    const float mine = __builtin_amdgcn_exp2f(st.m_run - m_use);
+    constexpr int CH = D / 4, CM = CH < 32 ? CH - 1 : 31;  // 16-byte chunk c of row r at c ^ (r & CM)
+    float* parts = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<f32x4*>(parts + (wave * PF_ROWS + col) * D +
+                                  (((dt * 8 + u * 2 + g) ^ (col & CM)) << 2)) =
+            f32x4{st.acc[dt][4 * u] * mine, st.acc[dt][4 * u + 1] * mine,
+                  st.acc[dt][4 * u + 2] * mine, st.acc[dt][4 * u + 3] * mine};
+    __syncthreads();
+    if (wave == 0 && g == 0) ml[0][col] = f32x2{m, l};  // to the threads that write the row
+    __syncthreads();
+    for (int i = tid; i < PF_ROWS * CH; i += 256) {
+      const int rr = i / CH, c = i % CH;
+      const int rq = w.it.tile * PF_ROWS + rr;
+      const int t = rq / a.group, h = hk * a.group + (rq - t * a.group);
+      if ((uint32_t)t >= (uint32_t)w.it.rows) continue;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(parts + (p * PF_ROWS + rr) * D +
+                                                        ((c ^ (rr & CM)) << 2));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += v[e];
+      }
+      const f32x2 x = ml[0][rr];
+      if (SPLIT && w.chunks > 1) {
+        const int64_t at = (int64_t)id * PF_ROWS + rr;
+        if (c == 0) a.stats[at] = f32x2{x[0], j_beg < j_end ? x[1] : -1.0f};
+        if (j_beg < j_end) *reinterpret_cast<f32x4*>(a.part + at * D + c * 4) = o;
+      } else {
+        const float inv = w.keys == 0 ? 0.f : 1.0f / x[1];
+        *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.o) + (int64_t)(w.it.row0 + t) * a.os[0] +
+                                  h * a.os[1] + c * 4) =
+            u32x2{MfmaT<T>::pack2(o[0] * inv, o[1] * inv), MfmaT<T>::pack2(o[2] * inv, o[3] * inv)};
+      }
+    }
+    if (!SPLIT) return;
+    __syncthreads();  // the next item's keys overwrite the parts
+  }
+}
+
+// The chunks of a row joined in their order: a workgroup per (row, head), each wavefront every fourth
+// chunk, a lane per chunk for the statistics, 64 at a time. (A sum of 0, all scores -inf, gives NaN
+// as it does whole.)
+template <typename T, int D, int BLOCK, int KEYT>
 __global__ __launch_bounds__(256) void packed_attn_join(const PackedAttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t heads = (int64_t)a.kv_heads * a.group;
-  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t all = a.rows_q * heads;
-  if (at >= all) return;
-  const int64_t row = at / heads, head = at - row * heads;
-  if (!a.zero_rest && !packed_covers(a.q_starts, a.requests, a.rows_q, (int)row)) return;
+  constexpr int PL = D / 64;  // channels per lane
+  __shared__ float parts[4][D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int heads = a.kv_heads * a.group;
+  const int row = blockIdx.x / heads, head = blockIdx.x - row * heads;
+  PackedChunks<BLOCK, KEYT> chunks;
+  chunks.scan(a);
+  const uint64_t in = __ballot(chunks.r0 <= row && row < chunks.r0 + chunks.len);
+  if (!in) return;
+  const PackedWork w = chunks.work_of(a, __ffsll((unsigned long long)in) - 1);
+  if (w.chunks <= 1) return;  // written where it was computed
+  const int hk = head / a.group, r = (row - w.it.row0) * a.group + head - hk * a.group;
+  const int tile = r / BLOCK;
+  // chunk p's slot and this row in it
+  const int64_t s0 = ((int64_t)(w.first + tile * w.chunks) * a.kv_heads + hk) * BLOCK + r - tile * BLOCK;
+  const int64_t step = (int64_t)a.kv_heads * BLOCK;
+  if (s0 + (w.chunks - 1) * step >= (int64_t)a.slots * BLOCK) return;
+  auto stats = [&](int c) {
+    return c + lane < w.chunks ? a.stats[s0 + (c + lane) * step] : f32x2{-INFINITY, -1.0f};
+  };
   float m = -INFINITY;
-  for (int p = 0; p < a.pieces; ++p) {
-    const f32x2 s = a.stats[p * all + at];
-    if (!(s[1] < 0.f)) m = fmaxf(m, s[0]);
+  for (int c = 0; c < w.chunks; c += kWave) {
+    const f32x2 s = stats(c);
+    m = fmaxf(m, wave_max(s[1] < 0.f ? -INFINITY : s[0]));
   }
   const float m_use = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[D / 64] = {};
-  bool any = false;
-  for (int p = 0; p < a.pieces; ++p) {
-    const f32x2 s = a.stats[p * all + at];
-    if (s[1] < 0.f) continue;
-    any = true;
-    const float w = __builtin_amdgcn_exp2f(s[0] - m_use);
-    l += w * s[1];
+  float l = 0.f, o[PL] = {};
+  for (int c = 0; c < w.chunks; c += kWave) {
+    const f32x2 s = stats(c);
+    const bool on = !(s[1] < 0.f);
+    const float wt = on ? __builtin_amdgcn_exp2f(s[0] - m_use) : 0.f;
+    l += wave_sum(on ? wt * s[1] : 0.f);
+    const uint64_t there = __ballot(on);
+    const int n = min(w.chunks - c, kWave);
+#pragma unroll 8
+    for (int p = wave; p < n; p += 4) {  // what a chunk without keys holds is not looked at
+      const float wp = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), p));
+      const float* q = a.part + (s0 + (c + p) * step) * D + lane * PL;
+      const bool use = (there >> p) & 1;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += w * a.part[(p * all + at) * D + i * 64 + lane];
+      for (int i = 0; i < PL; ++i) {
+        const float x = q[i];
+        o[i] += use ? wp * x : 0.f;
+      }
+    }
   }
-  const float inv = any ? 1.0f / l : 0.f;
-  T* op = reinterpret_cast<T*>(a.o) + row * a.os[0] + head * a.os[1];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) Elt<T>::store(op + i * 64 + lane, o[i] * inv);
+  for (int i = 0; i < PL; ++i) parts[wave][lane * PL + i] = o[i];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  const float sum = parts[0][d] + parts[1][d] + parts[2][d] + parts[3][d];
+  Elt<T>::store(reinterpret_cast<T*>(a.o) + row * a.os[0] + head * a.os[1] + d, sum * (1.0f / l));
 }
 
-static int packed_items(int64_t rows_q, int64_t requests, int64_t group, int64_t rows) {
-  return (int)((rows_q * group + rows - 1) / rows + requests + 2);
+// ------------------------------------------------------------------ host
+// What the host decides from the sizes it knows (never from the row numbers on the device).
+struct PackedPlan {
+  int block, key_tile;  // rows and keys of a tile
+  int items;            // row tiles per key head, at most
+  int groups;           // workgroups that cut keys into chunks; 0: keys stay whole
+  int64_t slots;        // chunks, at most
+};
+static PackedPlan packed_plan(int64_t rows_q, int64_t rows_k, int64_t requests, int64_t kv_heads,
+                              int64_t group) {
+  PackedPlan p = {};
+  // tiles of 32 rows where requests have fewer than 48 on average
+  const bool few = rows_q * group <= 48 * std::max<int64_t>(requests, 1);
+  p.block = few ? PF_ROWS : PA_ROWS;
+  p.key_tile = few ? PF_KEYS : PA_KEYS;
+  p.items = (int)((rows_q * group + p.block - 1) / p.block + requests + 2);
+  // two workgroups for each compute unit; launches of as many row tiles keep their keys whole
+  constexpr int kGroups = 512;
+  if (requests > 0 && requests <= PACKED_LANES && rows_k > p.key_tile &&
+      p.items * kv_heads < kGroups) {
+    p.groups = kGroups;
+    // PackedChunks::scan's count: at most `groups` and one for every row tile (and a few, for the
+    // rounding of its quotient)
+    p.slots = kGroups + p.items * kv_heads + 16;
+  }
+  return p;
 }
-
-// Pieces per request: enough workgroups to give every compute unit a few, as long as a piece keeps
-// two tiles of keys on average and the pieces' sums stay small beside the launch.
-static int packed_pieces(int64_t rows_q, int64_t rows_k, int64_t requests, int64_t kv_heads,
-                         int64_t group, int64_t head_dim) {
-  const int64_t blocks = packed_items(rows_q, requests, group, PA_ROWS) * kv_heads;
-  if (blocks >= 256) return 1;
-  int64_t n = (1024 + blocks - 1) / blocks;
-  n = std::min(n, (rows_k + 2 * PA_KEYS - 1) / (2 * PA_KEYS));
-  n = std::min<int64_t>(n, (16 << 20) / std::max<int64_t>(1, rows_q * kv_heads * group * head_dim * 4));
-  return (int)std::max<int64_t>(1, n);
+static int64_t packed_stats_bytes(const PackedPlan& p) {
+  return (p.slots * p.block * 8 + 255) / 256 * 256;
 }
-static int64_t packed_stats_bytes(int64_t pieces, int64_t rows_q, int64_t heads) {
-  return (pieces * rows_q * heads * 8 + 255) / 256 * 256;
+static int64_t packed_workspace(const PackedPlan& p, int64_t head_dim) {
+  return p.groups ? packed_stats_bytes(p) + p.slots * p.block * head_dim * 4 : 0;
 }
 
 }  // namespace dlt
@@ -297,11 +557,9 @@ extern "C" int64_t difflet_rocm_packed_attention_workspace_bytes(int64_t rows_q,
                                                                  int64_t kv_heads, int64_t group,
                                                                  int64_t head_dim) {
   if (rows_q <= 0 || rows_k <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 ||
-      rows_q * group >= (1LL << 30) || requests >= (1LL << 24) || kv_heads * group > 65536)
+      kv_heads * group > 65536 || rows_q * group >= (1LL << 30) || requests >= (1LL << 24))
     return 0;
-  const int64_t n = packed_pieces(rows_q, rows_k, requests, kv_heads, group, head_dim);
-  if (n <= 1) return 0;
-  return packed_stats_bytes(n, rows_q, kv_heads * group) + n * rows_q * kv_heads * group * head_dim * 4;
+  return packed_workspace(packed_plan(rows_q, rows_k, requests, kv_heads, group), head_dim);
 }
 
 extern "C" int difflet_rocm_packed_attention(
@@ -317,8 +575,9 @@ extern "C" int difflet_rocm_packed_attention(
               "%s: bf16 or fp16, not dtype %d", name, dtype);
   DLT_REQUIRE(head_dim == 64 || head_dim == 128, DIFFLET_EUNSUPPORTED,
               "%s: head_dim %lld (64 or 128)", name, (long long)head_dim);
-  DLT_REQUIRE(rows_q * group < (1LL << 30) && rows_k < (1LL << 30) && requests < (1LL << 24) &&
-                  kv_heads * group <= 65536,
+  DLT_REQUIRE(kv_heads <= 65536 && group <= 65536 && kv_heads * group <= 65536 &&
+                  rows_q < (1LL << 30) && rows_q * group < (1LL << 30) && rows_k < (1LL << 30) &&
+                  requests < (1LL << 24),
               DIFFLET_EUNSUPPORTED, "%s: too large", name);
   DLT_REQUIRE(scale - scale == 0.0f, DIFFLET_EINVAL, "%s: scale must be finite", name);
   if (rows_q == 0) return DIFFLET_OK;
@@ -329,9 +588,9 @@ extern "C" int difflet_rocm_packed_attention(
     DLT_REQUIRE(q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 &&
                     o_strides[i] % 4 == 0,
                 DIFFLET_EINVAL, "%s: rows and heads must start on 16 bytes (the output's on 8)", name);
-  DLT_REQUIRE(k_strides[0] >= 0 && v_strides[0] >= 0 && k_strides[0] < (1LL << 24) &&
-                  v_strides[0] < (1LL << 24),
-              DIFFLET_EUNSUPPORTED, "%s: key rows more than 32 MB apart", name);
+  DLT_REQUIRE(k_strides[0] >= 0 && v_strides[0] >= 0 && k_strides[0] <= (1LL << 23) &&
+                  v_strides[0] <= (1LL << 23),
+              DIFFLET_EUNSUPPORTED, "%s: key rows more than 16 MB apart", name);
   DLT_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((uintptr_t)o & 7) == 0,
               DIFFLET_EINVAL, "%s: misaligned pointers", name);
   PackedAttnArgs a = {};
@@ -357,35 +616,37 @@ extern "C" int difflet_rocm_packed_attention(
   // weighs any real score as 0 does
   a.scale_log2 = std::max((scale < 0 ? -scale : scale) * LOG2E, FLT_MIN);
   a.q_sign = scale < 0 ? 0x80008000u : 0u;
-  a.items = packed_items(rows_q, requests, group, PA_ROWS);
-  a.pieces = rows_k > 0 && requests > 0
-                 ? packed_pieces(rows_q, rows_k, requests, kv_heads, group, head_dim) : 1;
-  if (a.pieces > 1) {
-    const int64_t stats = packed_stats_bytes(a.pieces, rows_q, kv_heads * group);
-    const int64_t need = stats + a.pieces * rows_q * kv_heads * group * head_dim * 4;
-    if (!workspace || workspace_bytes < need) {
-      a.pieces = 1;  // without room for the pieces' sums the keys stay whole
-    } else {
-      DLT_REQUIRE(((uintptr_t)workspace & 255) == 0, DIFFLET_EINVAL,
-                  "%s: workspace must be 256-byte aligned", name);
-      a.stats = (f32x2*)workspace;
-      a.part = (float*)((uint8_t*)workspace + stats);
-    }
+  const PackedPlan plan = packed_plan(rows_q, rows_k, requests, kv_heads, group);
+  a.items = plan.items;
+  if (plan.groups && workspace && workspace_bytes >= packed_workspace(plan, head_dim)) {
+    DLT_REQUIRE(((uintptr_t)workspace & 255) == 0, DIFFLET_EINVAL,
+                "%s: workspace must be 256-byte aligned", name);
+    a.groups = plan.groups;
+    a.slots = (int)plan.slots;
+    a.stats = (f32x2*)workspace;
+    a.part = (float*)((uint8_t*)workspace + packed_stats_bytes(plan));
   }
-  const int64_t blocks = (int64_t)a.items * kv_heads * a.pieces;
+  const int64_t blocks = a.groups ? a.groups : (int64_t)a.items * kv_heads;
   DLT_REQUIRE(blocks < (1LL << 31), DIFFLET_EUNSUPPORTED, "%s: too many tiles", name);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)blocks), block(256);
   auto go = [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    if (a.pieces == 1) {
-      hipLaunchKernelGGL((packed_attn_kernel<T, D, false>), grid, block, 0, s, a);
+    const bool few = plan.block == PF_ROWS;
+    if (!a.groups) {
+      if (few) hipLaunchKernelGGL((packed_attn_few_kernel<T, D, false>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((packed_attn_kernel<T, D, false>), grid, block, 0, s, a);
       return;
     }
-    hipLaunchKernelGGL((packed_attn_kernel<T, D, true>), grid, block, 0, s, a);
-    const int64_t all = rows_q * kv_heads * group;
-    hipLaunchKernelGGL((packed_attn_join<T, D>), dim3((unsigned)((all + 3) / 4)), block, 0, s, a);
+    const dim3 rows((unsigned)(rows_q * kv_heads * group));
+    if (few) {
+      hipLaunchKernelGGL((packed_attn_few_kernel<T, D, true>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((packed_attn_join<T, D, PF_ROWS, PF_KEYS>), rows, block, 0, s, a);
+    } else {
+      hipLaunchKernelGGL((packed_attn_kernel<T, D, true>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((packed_attn_join<T, D, PA_ROWS, PA_KEYS>), rows, block, 0, s, a);
+    }
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

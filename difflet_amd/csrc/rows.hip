@@ -60,11 +60,12 @@ template <> struct Vec8<float> {
 // for two calls, this one stands for its formula. h is written out rounded to x's type (the next
 // residual stream); the norm takes the sum before that rounding.
 //
-// A row is held in registers by TPR threads (64: a wavefront; 256: a workgroup), so x and the
-// residual are read once. MX: a thread owns whole blocks of 32, whose elements are the four runs
-// k0 + j tile / 4 + 8 b + [0, 8) of a 512-wide tile (or the remainder): four 16-byte loads, 16
-// threads covering 256 consecutive bytes with each, and two 16-byte stores of codes in swizzle
-// order. Nothing crosses lanes but the row's sum and maximum.
+// A row is held in registers, so x and the residual are read once. MX: a thread owns a whole block
+// of 32, whose elements are the four runs k0 + j tile / 4 + 8 b + [0, 8) of a 512-wide tile (or the
+// remainder): four 16-byte loads, 16 threads covering 256 consecutive bytes with each, and two
+// 16-byte stores of codes in swizzle order; nothing crosses lanes but the row's sum (and maximum).
+// A workgroup takes a row with as many wavefronts as SLOTS units a thread leave (WG), or, where one
+// wavefront holds a row, four rows.
 struct RmsArgs {
   const void* x;
   const void* res;     // NULL: none
@@ -93,13 +94,22 @@ __device__ __forceinline__ int rms_run(int u, int j, int dim) {
   return k0 + j * sub + 8 * (u & 15);
 }
 
-template <typename T, bool MX, int TPR, int SLOTS>
-__global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
-  constexpr int RUNS = MX ? 4 : 1, RPW = 256 / TPR;  // runs of 8 per unit, rows per workgroup
-  __shared__ float red[4];
-  const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR;
-  if (TPR == 64 && row >= a.rows) return;  // TPR == 256: one row per workgroup, all there
+template <typename T, bool MX, bool WG, int SLOTS>
+__global__ __launch_bounds__(WG ? 1024 : 256) void rms_norm_quant_kernel(const RmsArgs a) {
+  constexpr int RUNS = MX ? 4 : 1;  // runs of 8 per unit
+  __shared__ float red[2][16];
+  const int tpr = WG ? blockDim.x : kWave;  // threads per row
+  const int t = WG ? threadIdx.x : threadIdx.x & (kWave - 1);
+  const int64_t row = WG ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (!WG && row >= a.rows) return;
+  auto over_row = [&](float v, float* slots, auto join) {  // v already joined over the wavefront
+    if constexpr (!WG) return v;
+    if ((threadIdx.x & (kWave - 1)) == 0) slots[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = slots[0];
+    for (int i = 1; i < (int)blockDim.x / kWave; ++i) v = join(v, slots[i]);
+    return v;
+  };
   const int units = a.dim / (8 * RUNS);
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
   const T* rr = a.res ? reinterpret_cast<const T*>(a.res) + row * a.ldr : nullptr;
@@ -107,7 +117,7 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
   float ss = 0.f;
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
-    const int u = s * TPR + t;
+    const int u = s * tpr + t;
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
       if (u < units) Vec8<T>::load(xr + rms_run<MX>(u, j, a.dim), v[s][j]);
@@ -120,7 +130,7 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
     T* hr = a.hidden ? reinterpret_cast<T*>(a.hidden) + row * a.ldh : nullptr;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      const int u = s * TPR + t;
+      const int u = s * tpr + t;
       if (u >= units) continue;
 #pragma unroll
       for (int j = 0; j < RUNS; ++j) {
@@ -138,12 +148,12 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
     for (int j = 0; j < RUNS; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[s][j][e], v[s][j][e], ss);
-  ss = block_sum<TPR / 64>(ss, red);
+  ss = over_row(wave_sum(ss), red[0], [](float p, float q) { return p + q; });
   const float rs = 1.0f / __fsqrt_rn(ss / (float)a.dim + a.eps);
   float amax = 0.f;
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
-    const int u = s * TPR + t;
+    const int u = s * tpr + t;
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
       float w[8];
@@ -166,13 +176,13 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) bad |= v[s][0][e] != v[s][0][e];
     amax = bad ? INFINITY : amax;
-    amax = block_max<TPR / 64>(amax, red);
+    amax = over_row(wave_max(amax), red[1], [](float p, float q) { return fmaxf(p, q); });
     const bool nan = amax == INFINITY;  // a finite row never reaches it: |y| <= sqrt(dim) |w|
     const float inv = nan ? __builtin_nanf("") : rowwise_inv(amax);
     if (t == 0) reinterpret_cast<float*>(a.scales)[row] = nan ? inv : rowwise_scale(amax);
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      const int u = s * TPR + t;
+      const int u = s * tpr + t;
       if (u >= units) continue;
       *reinterpret_cast<u32x2*>(qr + u * 8) =
           nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : encode8_rowwise(v[s][0], inv);
@@ -181,7 +191,7 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
     uint8_t* sr = reinterpret_cast<uint8_t*>(a.scales) + row * a.lds;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      const int u = s * TPR + t;
+      const int u = s * tpr + t;
       if (u >= units) continue;
       uint32_t emax = 0;
       bool bad = false;
@@ -215,40 +225,16 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const RmsArgs a) {
 
 template <typename T, bool MX>
 static void launch_rms(const RmsArgs& a, hipStream_t s) {
-  constexpr int UNIT = MX ? 32 : 8;
-  const int units = a.dim / UNIT;
-  // a wavefront per row where rows fill the chip, a workgroup where they are few or wide
-  const bool wave = a.rows >= 1024 && a.dim <= 6144;
-  const dim3 block(256);
-#define DLT_RMS(TPR, N)                                                                       \
-  hipLaunchKernelGGL((rms_norm_quant_kernel<T, MX, TPR, N>),                                  \
-                     dim3((unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR))), block, 0, s, a)
-  if (wave) {
-    const int slots = (units + 63) / 64;
-    if constexpr (MX) {
-      if (slots <= 1) DLT_RMS(64, 1);
-      else if (slots <= 2) DLT_RMS(64, 2);
-      else DLT_RMS(64, 3);
-    } else {
-      if (slots <= 4) DLT_RMS(64, 4);
-      else if (slots <= 6) DLT_RMS(64, 6);
-      else if (slots <= 8) DLT_RMS(64, 8);
-      else if (slots <= 10) DLT_RMS(64, 10);
-      else DLT_RMS(64, 12);
-    }
-  } else {
-    const int slots = (units + 255) / 256;
-    if constexpr (MX) {
-      if (slots <= 1) DLT_RMS(256, 1);
-      else DLT_RMS(256, 2);
-    } else {
-      if (slots <= 1) DLT_RMS(256, 1);
-      else if (slots <= 2) DLT_RMS(256, 2);
-      else if (slots <= 4) DLT_RMS(256, 4);
-      else DLT_RMS(256, 8);
-    }
-  }
-#undef DLT_RMS
+  // one unit (MX) or two (rows) a thread keep registers few and the loads of many rows in flight:
+  // 32760 x 5120 MXFP8 in NORM_A us, NORM_B with a wavefront per row and three units a thread
+  constexpr int SLOTS = MX ? 1 : 2;
+  const int units = a.dim / (MX ? 32 : 8), waves = (units + SLOTS * kWave - 1) / (SLOTS * kWave);
+  if (waves > 1)
+    hipLaunchKernelGGL((rms_norm_quant_kernel<T, MX, true, SLOTS>), dim3((unsigned)a.rows),
+                       dim3((unsigned)(waves * kWave)), 0, s, a);
+  else
+    hipLaunchKernelGGL((rms_norm_quant_kernel<T, MX, false, SLOTS>),
+                       dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 // ------------------------------------------------------------------ rotary positions
