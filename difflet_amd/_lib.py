@@ -151,13 +151,14 @@ SIGNATURES: dict[str, tuple] = {
     "difflet_rocm_rows_to_planes": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _f32, _f32, _vp]),
     "difflet_rocm_rms_norm_quant": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
                                            _i32, _i64, _i64, _vp, _i32, _f32, _i32, _vp]),
-    "difflet_rocm_rope_axes": (_i32, [_vp, _vp, _i64p, _i64p, _i64, _vp, _vp, _i64p, _i64p, _i64,
-                                      _i32, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _i64, _vp,
-                                      _vp, _i32, _vp]),
+    # the strides of these two go as addresses: several in one host array
+    "difflet_rocm_rope_axes": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i64,
+                                      _i64, _i64, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32,
+                                      _vp]),
     "difflet_rocm_packed_attention_workspace_bytes": (_i64, [_i64] * 6),
     "difflet_rocm_packed_attention": (_i32, [
-        _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _vp,
-        _vp, _i64, _f32, _i32, _vp, _i64, _vp]),
+        _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+        _f32, _i32, _vp, _i64, _vp]),
     "difflet_rocm_lora_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64]),
     "difflet_rocm_lora_linear": (_i32, [
         _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp,

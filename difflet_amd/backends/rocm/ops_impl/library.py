@@ -297,6 +297,9 @@ def _(x, cos, sin, law):
 
 
 # ---------------------------------------------------------------------------- packed requests
+# Called with single tokens, where a trip through the dispatcher (4 us) would be a fifth of the call:
+# in plain eager inference, which is what _inference() says, the implementations are called as they
+# are. Everything else goes to the custom_op, whose backward refuses.
 def _rms_norm_quant_impl(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
                          eps: float, mx: bool) -> tuple[Tensor, Tensor, Tensor]:
     """difflet_rocm_rms_norm_quant on x [rows, dim]: (codes, scales, x + residual, which is empty
@@ -316,13 +319,12 @@ def _rms_norm_quant_fake(x, weight, residual, eps, mx):
 _rms_norm_quant_op = torch.library.custom_op("difflet_rocm::rms_norm_quant", _rms_norm_quant_impl,
                                              mutates_args=())
 _rms_norm_quant_op.register_fake(_rms_norm_quant_fake)
-_rms_norm_quant_infer = _infer_twin(_rms_norm_quant_op, _rms_norm_quant_impl, _rms_norm_quant_fake)
 
 
 def rms_norm_quant(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float,
                    mx: bool) -> tuple[Tensor, Tensor, Tensor]:
     if _inference(x, weight, residual):
-        return _rms_norm_quant_infer.redispatch(_DEVICE, x, weight, residual, eps, mx)
+        return _rms_norm_quant_impl(x, weight, residual, eps, mx)
     return _rms_norm_quant_op(x, weight, residual, eps, mx)
 
 
@@ -339,13 +341,12 @@ def _rope_axes_fake(q, k, positions, axes, theta, halves, shared):
 
 _rope_axes_op = torch.library.custom_op("difflet_rocm::rope_axes", _rope_axes_impl, mutates_args=())
 _rope_axes_op.register_fake(_rope_axes_fake)
-_rope_axes_infer = _infer_twin(_rope_axes_op, _rope_axes_impl, _rope_axes_fake)
 
 
 def rope_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, axes: list[int], theta: float,
               halves: bool, shared: bool) -> tuple[Tensor, Tensor]:
     if _inference(q, k, positions):
-        return _rope_axes_infer.redispatch(_DEVICE, q, k, positions, axes, theta, halves, shared)
+        return _rope_axes_impl(q, k, positions, axes, theta, halves, shared)
     return _rope_axes_op(q, k, positions, axes, theta, halves, shared)
 
 
@@ -362,14 +363,12 @@ def _packed_attention_fake(q, k, v, q_starts, k_starts, scale):
 _packed_attention_op = torch.library.custom_op("difflet_rocm::packed_attention",
                                                _packed_attention_impl, mutates_args=())
 _packed_attention_op.register_fake(_packed_attention_fake)
-_packed_attention_infer = _infer_twin(_packed_attention_op, _packed_attention_impl,
-                                      _packed_attention_fake)
 
 
 def packed_attention(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts: Tensor,
                      scale: float) -> Tensor:
     if _inference(q, k, v, q_starts, k_starts):
-        return _packed_attention_infer.redispatch(_DEVICE, q, k, v, q_starts, k_starts, scale)
+        return _packed_attention_impl(q, k, v, q_starts, k_starts, scale)
     return _packed_attention_op(q, k, v, q_starts, k_starts, scale)
 
 
@@ -397,14 +396,12 @@ def _lora_linear_fake(x, w, w_scale, bias, down, up, scale, starts, ids):
 _lora_linear_op = torch.library.custom_op("difflet_rocm::lora_linear", _lora_linear_impl,
                                           mutates_args=())
 _lora_linear_op.register_fake(_lora_linear_fake)
-_lora_linear_infer = _infer_twin(_lora_linear_op, _lora_linear_impl, _lora_linear_fake)
 
 
 def lora_linear(x: Tensor, w: Tensor, w_scale: Optional[Tensor], bias: Optional[Tensor],
                 down: Tensor, up: Tensor, scale: Tensor, starts: Tensor, ids: Tensor) -> Tensor:
     if _inference(x, w, w_scale, bias, down, up, scale, starts, ids):
-        return _lora_linear_infer.redispatch(_DEVICE, x, w, w_scale, bias, down, up, scale, starts,
-                                             ids)
+        return _lora_linear_impl(x, w, w_scale, bias, down, up, scale, starts, ids)
     return _lora_linear_op(x, w, w_scale, bias, down, up, scale, starts, ids)
 
 

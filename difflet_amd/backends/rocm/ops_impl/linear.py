@@ -160,11 +160,10 @@ def lora_linear(x, weight, bias, down, up, scale, row_starts, adapter, *, weight
     if down.dim() != 3 or down.shape[2] != k or up.dim() != 3 or up.shape[1] != n:
         raise ValueError(f"adapters of this weight are down [adapters, rank, {k}] and up [adapters, "
                          f"{n}, rank], got {tuple(down.shape)} and {tuple(up.shape)}")
-    x2 = x.reshape(-1, k)
     b = None if bias is None else bias.detach().to(torch.bfloat16)
-    y = library.lora_linear(x2.to(torch.bfloat16), weight, weight_scale, b, down, up, scale,
-                            row_starts, adapter)
-    return y.reshape(*x.shape[:-1], n).to(x.dtype)
+    x2 = (x if x.dim() == 2 else x.reshape(-1, k)).to(torch.bfloat16)
+    y = library.lora_linear(x2, weight, weight_scale, b, down, up, scale, row_starts, adapter)
+    return (y if x.dim() == 2 else y.reshape(*x.shape[:-1], n)).to(x.dtype)
 
 
 class ParallelEmbedding(nn.Embedding):

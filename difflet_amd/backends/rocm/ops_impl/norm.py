@@ -53,6 +53,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor | None, eps: float,
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must be {x.dtype} {tuple(x.shape)}, got {residual.dtype} "
                          f"{tuple(residual.shape)}")
+    if x.dim() == 2:
+        q, s, h = library.rms_norm_quant(x, weight, residual, float(eps), mx)
+        return q, s, x if residual is None else h
     r2 = None if residual is None else residual.reshape(-1, dim)
     q, s, h = library.rms_norm_quant(x.reshape(-1, dim), weight, r2, float(eps), mx)
     lead = x.shape[:-1]

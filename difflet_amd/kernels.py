@@ -7,7 +7,6 @@ Outputs are allocated with torch (the library never allocates).
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
@@ -1181,16 +1180,38 @@ def rows_to_planes(x: torch.Tensor, channels: int, *, lo: float = float("-inf"),
 
 
 # ------------------------------------------------------------------------ packed requests
-def _current(dev: torch.device):
-    """A context in which dev is the current device, as a launch on its streams needs."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+# These operators are called with few rows, where the host's time is the call's: pointers go as plain
+# numbers, strides as one array.
+def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The one device of these tensors, as _on_gpu (whose messages it leaves the refusals to)."""
+    i = first.get_device()
+    if i < 0 or any(t is not None and t.get_device() != i for t in others):
+        return _on_gpu(first, *others)
+    return first.device
+
+
+def _launch(dev: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, the device's current stream), with dev the current device as its streams need."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if st:
+        check(st, what)
+
+
+def _p(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+_I64x8, _I64x12 = ctypes.c_int64 * 8, ctypes.c_int64 * 12
 
 
 def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
     """t as [rows, cols] rows that start on 16 bytes, a copy where they do not."""
-    t2 = _rows2d(t, name)
+    t2 = t if t.dim() == 2 and t.stride(1) == 1 else _rows2d(t, name)
     if t2.stride(0) % 8 or t2.data_ptr() % 16:
         t2 = t2.clone(memory_format=torch.contiguous_format)
     return t2
@@ -1211,7 +1232,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
     [rows, dim], scales, h in x's dtype [rows, dim], x itself without a residual). Scales: fp32
     [rows], or with mx E8M0 uint8 [rows, dim / 32], codes and blocks in swizzle order. hidden: where
     to write h (x and residual may be given). dim a multiple of 8 (mx: 128), at most 16384."""
-    dev = _on_gpu(x, weight, residual, hidden)
+    dev = _device_of(x, weight, residual, hidden)
     if x.dtype not in FLOAT_DTYPES:
         raise TypeError(f"rms_norm_quant: x must be bf16, fp16 or fp32, got {x.dtype}")
     dim = x.shape[-1]
@@ -1239,13 +1260,11 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
     q = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=dev)
     s = torch.empty((rows, dim // 32) if mx else (rows,),
                     dtype=torch.uint8 if mx else torch.float32, device=dev)
-    with _current(dev):
-        check(lib().difflet_rocm_rms_norm_quant(
-            _ptr(x2), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(hidden),
-            0 if hidden is None else max(hidden.stride(0), dim), _ptr(q), dim, _ptr(s),
-            dim // 32 if mx else 0, _dt(x), rows, dim, _ptr(weight),
-            _lib.F32 if weight is None else _dt(weight), float(eps), int(mx), _stream(dev)),
-            "rms_norm_quant")
+    _launch(dev, "rms_norm_quant", lib().difflet_rocm_rms_norm_quant, x2.data_ptr(), x2.stride(0),
+            _p(r2), 0 if r2 is None else r2.stride(0), _p(hidden),
+            0 if hidden is None else max(hidden.stride(0), dim), q.data_ptr(), dim, s.data_ptr(),
+            dim // 32 if mx else 0, _DT[x.dtype], rows, dim, _p(weight),
+            0 if weight is None else _DT[weight.dtype], eps, int(mx))
     return q, s, x2 if hidden is None else hidden
 
 
@@ -1272,7 +1291,7 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     """Rotary embedding of q [batch, seq, heads, dim] and k (heads of its own, or None) from
     positions [batch or 1, seq, len(axes)] (int32, int64 or fp32): axis a turns axes[a] channels.
     q_out, k_out: where to write (the inputs may be given); new contiguous tensors without."""
-    dev = _on_gpu(q, k, positions, q_out, k_out)
+    dev = _device_of(q, k, positions, q_out, k_out)
     axes = tuple(int(d) for d in axes)
     if not 1 <= len(axes) <= 8 or any(d < 2 or d % 2 for d in axes):
         raise ValueError(f"rope_axes: 1 to 8 axes of an even number of channels each, got {axes}")
@@ -1315,17 +1334,14 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     q, q_out = prepared(q, q_out, "q_out")
     k, k_out = prepared(k, k_out, "k_out")
     turns, axis = _rope_pairs(axes, float(theta), bool(shared))
-    args = []
-    for t, o in ((q, q_out), (k, k_out)):
-        if t is None:
-            args += [None, None, None, None, 0]
-        else:
-            args += [_ptr(t), _ptr(o), _arr(t.stride()[:3]), _arr(o.stride()[:3]), t.shape[2]]
-    with _current(dev):
-        check(lib().difflet_rocm_rope_axes(
-            *args, _dt(q), b, s, d, _ptr(positions), _POSITIONS[positions.dtype],
+    strides = _I64x12(*q.stride()[:3], *q_out.stride()[:3],
+                      *(() if k is None else (*k.stride()[:3], *k_out.stride()[:3])))
+    at = ctypes.addressof(strides)
+    _launch(dev, "rope_axes", lib().difflet_rocm_rope_axes, q.data_ptr(), q_out.data_ptr(), at,
+            at + 24, q.shape[2], _p(k), _p(k_out), at + 48, at + 72, 0 if k is None else k.shape[2],
+            _DT[q.dtype], b, s, d, positions.data_ptr(), _POSITIONS[positions.dtype],
             positions.stride(0) if positions.shape[0] > 1 else 0, len(axes), sum(axes) // 2, turns,
-            axis, int(halves), _stream(dev)), "rope_axes")
+            axis, int(halves))
     return q_out, k_out
 
 
@@ -1342,13 +1358,10 @@ def _starts(t: torch.Tensor, requests: int | None, name: str) -> int:
 
 def _heads16(t: torch.Tensor) -> torch.Tensor:
     """t [rows, heads, dim] with contiguous heads that start on 16 bytes, a copy where they do not."""
-    ok = (t.shape[2] == 1 or t.stride(2) == 1) and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or st % 8 == 0 for n, st in zip(t.shape[:2], t.stride()[:2]))
+    (rows, heads, dim), (sr, sh, sd) = t.shape, t.stride()
+    ok = ((sd == 1 or dim == 1) and t.data_ptr() % 16 == 0 and (sr % 8 == 0 or rows <= 1)
+          and (sh % 8 == 0 or heads <= 1))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def _row_head(t: torch.Tensor):
-    return _arr([st if n > 1 else 0 for n, st in zip(t.shape[:2], t.stride()[:2])])
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor,
@@ -1359,7 +1372,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
     q_starts[i + 1] - 1 and states k_starts[i] .. k_starts[i + 1] - 1 (int32 on the device, not read
     by the host). A request without states has zero rows; rows of no request are zero, in a given
     `out` left as they are."""
-    dev = _on_gpu(q, k, v, q_starts, k_starts, out)
+    dev = _device_of(q, k, v, q_starts, k_starts, out)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
         raise ValueError(f"packed_attention: q [rows, heads, dim] with k and v [states, key heads, "
                          f"dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -1380,15 +1393,22 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
             raise ValueError(f"packed_attention: out must be {q.dtype} {tuple(q.shape)} with heads "
                              "that start on 8 bytes and do not overlap")
     q, k, v = _heads16(q), _heads16(k), _heads16(v)
-    with _current(dev):
-        nbytes = lib().difflet_rocm_packed_attention_workspace_bytes(rows, k.shape[0], n, hk,
-                                                                     h // hk, d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(lib().difflet_rocm_packed_attention(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(o), _dt(q), rows, k.shape[0], hk, h // hk, d,
-            _row_head(q), _row_head(k), _row_head(v), _row_head(o), _ptr(q_starts), _ptr(k_starts),
-            n, float(scale), int(out is None), _ptr(ws), nbytes, _stream(dev)), "packed_attention")
+    states = k.shape[0]
+    # the stride of a dimension of one (or none) says nothing
+    strides = _I64x8(*(st if m > 1 else 0 for t in (q, k, v, o)
+                       for m, st in zip(t.shape[:2], t.stride()[:2])))
+    at = ctypes.addressof(strides)
+    nbytes = lib().difflet_rocm_packed_attention_workspace_bytes(rows, states, n, hk, h // hk, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(dev, "packed_attention", lib().difflet_rocm_packed_attention, q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), o.data_ptr(), _dt(q), rows, states, hk, h // hk, d, at, at + 16, at + 32,
+            at + 48, q_starts.data_ptr(), k_starts.data_ptr(), n, scale, int(out is None), _p(ws),
+            nbytes)
     return o
+
+
+def _lora_operand(x: torch.Tensor, kind: str):
+    return quantize_mxfp8(x, swizzled=True) if kind == "mx" else quantize_fp8_rowwise(x)
 
 
 def lora_linear(kind: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None,
@@ -1400,7 +1420,7 @@ def lora_linear(kind: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor 
     no request have none. kind and w, w_scale as gemm_call's (K and N its multiples); down bf16
     [adapters, rank, <= K], up bf16 [adapters, <= N, rank], scale fp32 [adapters], starts and ids
     int32 on the device. prepared: x's codes and scales for the fp8 kinds, quantized here without."""
-    dev = _on_gpu(x, w, bias, down, up, scale, starts, ids, w_scale)
+    dev = _device_of(x, w, bias, down, up, scale, starts, ids, w_scale)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"lora_linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not chain")
     m, k = x.shape
@@ -1442,27 +1462,28 @@ def lora_linear(kind: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor 
         x, w = _near_rows(x), _near_rows(w)
     kid = _KIND_ID[kind]
     a, a_scale = x, None
-    with _current(dev):
-        if kid:
-            if prepared is not None:
-                a, a_scale = prepared
-            else:
-                a, a_scale = (quantize_mxfp8(x, swizzled=True) if kind == "mx"
-                              else quantize_fp8_rowwise(x))
-            _check_epilogue_operands(Problem(a, w, y, None, a_scale=a_scale, w_scale=w_scale), 0,
-                                     kind, n, k, _lib.EPI_NONE)
-            if a.shape != (m, k) or a.stride(1) != 1 or a.dtype not in _GEMM_A_DTYPES[kind] or \
-                    w.dtype not in _GEMM_A_DTYPES[kind]:
-                raise ValueError(f"lora_linear: {kind} weights are e4m3 codes, prepared e4m3 codes "
-                                 f"[{m}, {k}]")
-            _on_gpu(x, a, a_scale, w_scale)
-        elif w.dtype != torch.bfloat16:
-            raise TypeError(f"lora_linear: bf16 weights, got {w.dtype}")
-        nbytes = lib().difflet_rocm_lora_workspace_bytes(kid, m, n, k, rank, requests)
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-        check(lib().difflet_rocm_lora_linear(
-            kid, _ptr(a), a.stride(0), _ptr(a_scale), _ptr(w), w.stride(0), _ptr(w_scale),
-            _ptr(bias), _ptr(y), n, m, n, k, _ptr(x), x.stride(0), kd, _ptr(down), _ptr(up),
-            up.shape[1], _ptr(scale), adapters, rank, _ptr(starts), _ptr(ids), requests, _ptr(ws),
-            ws.numel(), _stream(dev)), "lora_linear")
+    if kid:
+        if prepared is not None:
+            a, a_scale = prepared
+            _device_of(x, a, a_scale)
+        elif dev.index == torch.cuda.current_device():
+            a, a_scale = _lora_operand(x, kind)
+        else:
+            with torch.cuda.device(dev):
+                a, a_scale = _lora_operand(x, kind)
+        _check_epilogue_operands(Problem(a, w, y, None, a_scale=a_scale, w_scale=w_scale), 0, kind, n,
+                                 k, _lib.EPI_NONE)
+        if a.shape != (m, k) or a.stride(1) != 1 or a.dtype not in _GEMM_A_DTYPES[kind] or \
+                w.dtype not in _GEMM_A_DTYPES[kind]:
+            raise ValueError(f"lora_linear: {kind} weights are e4m3 codes, prepared e4m3 codes "
+                             f"[{m}, {k}]")
+    elif w.dtype != torch.bfloat16:
+        raise TypeError(f"lora_linear: bf16 weights, got {w.dtype}")
+    nbytes = lib().difflet_rocm_lora_workspace_bytes(kid, m, n, k, rank, requests)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+    _launch(dev, "lora_linear", lib().difflet_rocm_lora_linear, kid, a.data_ptr(), a.stride(0),
+            _p(a_scale), w.data_ptr(), w.stride(0), _p(w_scale), _p(bias), y.data_ptr(), n, m, n, k,
+            x.data_ptr(), x.stride(0), kd, down.data_ptr(), up.data_ptr(), up.shape[1],
+            scale.data_ptr(), adapters, rank, starts.data_ptr(), ids.data_ptr(), requests,
+            ws.data_ptr(), ws.numel())
     return y
