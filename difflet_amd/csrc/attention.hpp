@@ -64,6 +64,14 @@ __device__ __forceinline__ void dma16(i32x4_t r, const uint8_t* lds_ptr, uint32_
                : "s"(la), "v"(voff), "s"(r)
                : "memory", "m0");
 }
+// The same with a scalar offset beside the lanes' own.
+__device__ __forceinline__ void dma16s(i32x4_t r, const uint8_t* lds_ptr, uint32_t voff, uint32_t soff) {
+  const uint32_t la = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_t*)lds_ptr);
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(la), "v"(voff), "s"(r), "s"(soff)
+               : "memory", "m0");
+}
 // The words of make_rsrc's resource: base address, stride 0, `bytes` records, the same flags.
 __device__ __forceinline__ i32x4_t rsrc_words(const void* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);

@@ -10,6 +10,8 @@
 // feeds the second product from registers, as in attention.hip. Buffer ranges end with the
 // request's last key: rows of the next request or past the tensor read as zero, whatever lies there.
 //
+// Which one runs is packed_plan's choice.
+// packed_attn_wide_kernel: 256 rows, 64 a wavefront, where there are many (described beside it).
 // packed_attn_kernel: 128 rows (four wavefronts of 32), tiles of 64 keys through two LDS buffers, K
 // row-major, V transposed while it is written.
 // packed_attn_few_kernel: few rows a request (single tokens): 32 rows, whose four wavefronts take 32
@@ -19,7 +21,7 @@
 // about one length, one or two a workgroup (the length follows from the row numbers on the
 // device). A row tile of several chunks leaves the unnormalized sums of each and their statistics in
 // the workspace, joined by packed_attn_join in the order of the chunks. 16 single tokens over 0 to
-// 8000 states (4 key heads): 28 + 6 us with every request's keys in 12 pieces, CHUNK_A us so.
+// 8000 states (4 key heads): 28 + 6 us with every request's keys in 12 pieces, 24 + 5.7 so.
 #include <float.h>
 
 #include <algorithm>
@@ -27,7 +29,10 @@
 #include "attention.hpp"
 #include "packed.hpp"
 
+
 namespace dlt {
+
+int gemm_device_cus();  // compute units of the current device (gemm.hip)
 
 struct PackedAttnArgs {
   const uint8_t* q;
@@ -40,6 +45,7 @@ struct PackedAttnArgs {
   int requests, rows_q, rows_k, kv_heads, group;
   int items;         // row tiles per key head, at most
   int zero_rest;     // rows of no request come out zero (else are not written)
+  uint32_t group_m;  // conv_magic(group)
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // 0x80008000 for a negative scale
   int groups;           // workgroups of a launch that cuts keys into chunks (0: whole keys)
@@ -59,7 +65,7 @@ struct PackedWork {
 
 __device__ __forceinline__ void packed_keys(const PackedAttnArgs& a, int i, int& kbeg, int& keys) {
   kbeg = 0, keys = 0;
-  if (i < a.requests) {
+  if ((uint32_t)i < (uint32_t)a.requests) {
     kbeg = packed_start(a.k_starts, i, a.rows_k);
     keys = max(packed_start(a.k_starts, i + 1, a.rows_k) - kbeg, 0);
   }
@@ -71,11 +77,17 @@ constexpr int PACKED_LANES = kWave - 2;
 template <int BLOCK, int KEYT> struct PackedChunks {
   int r0, len, kbeg, keys;  // the lane's request (or rows of none)
   int tiles, chunks, upto;  // row tiles, chunks of each; items up to and with the lane's
-  __device__ __forceinline__ void scan(const PackedAttnArgs& a) {
+  // every request's keys in one chunk
+  __device__ __forceinline__ void load(const PackedAttnArgs& a) {
     const int i = threadIdx.x & (kWave - 1);
     packed_rows(a.q_starts, a.requests, a.rows_q, a.zero_rest != 0, i, r0, len);
     packed_keys(a, i, kbeg, keys);
     tiles = (len * a.group + BLOCK - 1) / BLOCK;
+    chunks = 1;
+    upto = wave_prefix(tiles);
+  }
+  __device__ __forceinline__ void scan(const PackedAttnArgs& a) {
+    load(a);
     const int kt = (keys + KEYT - 1) / KEYT;
     // key tiles per chunk, so that the chunks of all heads, a last short one for every row tile among
     // them, are one a workgroup (a schedule: every wavefront rounds alike, and that is all it takes)
@@ -274,6 +286,13 @@ template <typename T, int D> struct PackedRow {
   }
 };
 
+// Workgroup barrier after this wavefront's direct-to-LDS loads have landed but for the VM newest.
+template <int VM = 0> __device__ __forceinline__ void wide_barrier() {
+  static_assert(VM >= 0 && VM < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (VM & 15) | ((VM >> 4) << 14));  // vmcnt(VM) lgkmcnt(0)
+  asm volatile("s_barrier" ::: "memory");
+}
+
 // ------------------------------------------------------------------ kernels
 constexpr int PA_ROWS = 128, PA_KEYS = 64;
 
@@ -349,6 +368,424 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(const PackedAttnArg
                     MfmaT<T>::pack2(st.acc[dt][4 * u + 2] * inv, st.acc[dt][4 * u + 3] * inv)};
     }
     if (!SPLIT) return;
+  }
+}
+
+// Many rows a request: 256 rows a workgroup, 64 a wavefront in two column groups, one workgroup a
+// compute unit that walks tile after tile. Attention of many rows to a few hundred keys is bound by
+// the matrix cores (at the power they draw, about 1.26 PFLOP/s of the 2.5), if the softmax, the LDS
+// and the start and end of each tile stay beside them. On the 128-row kernel a fragment read feeds
+// one MFMA (the LDS's 128 bytes a cycle, all of them) and each tile begins and ends by itself. Here a
+// fragment feeds two MFMAs, the keys serve 256 rows, and one wavefront overlaps three halves (32
+// keys) of its work by itself: while the matrix core runs the scores of half h + 1 and the second
+// product of half h - 1, 32 MFMAs, the VALU takes the exponentials of half h. Four wavefronts with
+// 512 registers each hold the 128 accumulators, two sets of scores and of P and the rows' Q.
+//
+// Keys and values come straight from memory into LDS, two tiles of 64 keys each, K rows of D / 8 +
+// 1 slots of 16 bytes, V rows of 20 (12 for 64 channels), read through the transposing LDS read; slots
+// past the channels are padding that keeps the reads of 16 rows in distinct banks. Tile j's keys are
+// read in halves 2j - 1 and 2j, its values in 2j + 1 and 2j + 2, so one barrier a tile, before half
+// 2j - 1, publishes K(j) and V(j - 1) and frees the slots of K(j - 1) and V(j - 2), to which K(j + 1)
+// and V(j) go. Rows past the request's last key load that key again: their scores are masked to
+// -inf and what their P of 0 meets is as finite as the key's own values are. The next row tile's Q
+// comes the same way, a quarter of it with each tile of keys, and its first keys under the last half:
+// nothing of a tile's start is waited for but what a request of few keys leaves no time for.
+//
+// Exponentials are relative to a reference that moves to the running maximum when a lane's sum of
+// a half reaches the type's limit (the first half always): the statistics cost no maximum on the way.
+//
+// Rows of Q are fetched whole, 256 bytes a row: read as fragments, 32 rows at the stride of all
+// heads share a few sets of the L1, and each line comes four times. For the same reason the result goes
+// out through LDS (stored from the accumulators, 32 bytes of 32 rows an instruction, it took
+// 5,400 cycles a tile, so 4,000).
+//
+// 32,768 rows of 40 heads to 64, 128, 256, 512, 1024, 2048 keys: 165, 212, 285, 474, 831, 1474 us
+// (0.93 PFLOP/s); tiles of 128 rows: 246, 271, 356, 538, 873, 1575. Of the 49,000 cycles of a tile of 512
+// keys its loop takes 37,500, 5,360 a tile of keys (64 MFMAs a wavefront, 4,100 at the rate they
+// have alone).
+template <int D> struct WideLds {
+  static constexpr int KS = D / 8 + 1, VS = D == 128 ? 20 : 12;  // slots of 16 bytes per row
+  static constexpr int KB = 64 * KS * 16, VB = 64 * VS * 16;     // bytes per tile: KS, VS loads of 1 KB
+  static constexpr int QB = 64 * D * 2;                          // a wavefront's rows of Q
+  static constexpr int QL = QB / 1024, QQ = QL / 4;              // loads of it, a quarter
+  static constexpr int STORES = D / 8;                           // of a wavefront's output
+  static constexpr int BYTES = 2 * (KB + VB) + 4 * QB + 4 * 4096;
+};
+constexpr int PW_ROWS = 256;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void packed_attn_wide_kernel(const PackedAttnArgs a) {
+  typedef typename MfmaT<T>::frag frag;
+  typedef WideLds<D> L;
+  constexpr int NC = D / 16, NDT = D / 32, RPL = D / 8;  // RPL: 16-byte chunks a row
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, g = lane >> 5;
+  uint8_t* qlds = lds + 2 * (L::KB + L::VB) + wave * L::QB;
+  auto kbuf = [&](int b) { return lds + b * L::KB; };
+  auto vbuf = [&](int b) { return lds + 2 * L::KB + b * L::VB; };
+
+  // the requests, one a lane, and how many row tiles there are up to and with the lane's when those
+  // of most keys come first: the launch's last round, which its workgroups share unevenly, is then
+  // of short ones, and no tile costs another load to find
+  PackedChunks<PW_ROWS, 64> reqs;
+  reqs.load(a);
+  int upto = 0, tiles = 0;
+  for (int l = 0; l < a.requests + 2; ++l) {
+    const int k = __builtin_amdgcn_readlane(reqs.keys, l), n = __builtin_amdgcn_readlane(reqs.tiles, l);
+    if (k > reqs.keys || (k == reqs.keys && l <= lane)) upto += n;
+    tiles += n;
+  }
+  struct Tile {
+    PackedWork w;
+    int hk, nt;
+  };
+  auto find = [&](int64_t n) {
+    Tile t = {};
+    t.w.it.req = -1;
+    if (n >= (int64_t)tiles * a.kv_heads) return t;
+    const int64_t end = (int64_t)upto * a.kv_heads, begin = end - (int64_t)reqs.tiles * a.kv_heads;
+    const int l = __ffsll((unsigned long long)__ballot(begin <= n && n < end)) - 1;
+    t.w = reqs.work_of(a, l);
+    const int of = __builtin_amdgcn_readlane(reqs.tiles, l);
+    const int in = (int)(n - (int64_t)(__builtin_amdgcn_readlane(upto, l) - of) * a.kv_heads);
+    t.hk = in / of;
+    t.w.it.tile = in - t.hk * of;
+    t.nt = (t.w.keys + 63) / 64;
+    return t;
+  };
+  // load i of a wavefront's rows of Q: RPI rows, the lane's chunk lane % RPL of LDS row r holds chunk
+  // (lane % RPL) ^ (r % RPL) of it; rows past the request are its last. A load's offsets cost more
+  // than the load, so whole tiles of single heads step from the first one's
+  constexpr int RPI = 64 / RPL;
+  const bool single = a.group == 1;
+  const uint32_t qrow = (uint32_t)(a.qs[0] * 2);
+  auto q_offset = [&](const Tile& t, int i, uint32_t tok0) {
+    const int r = i * RPI + lane / RPL, last = t.w.it.rows * a.group - 1;
+    uint32_t h;
+    const uint32_t tok = conv_udiv((uint32_t)min(t.w.it.tile * PW_ROWS + wave * 64 + r, last),
+                                   (uint32_t)a.group, a.group_m, h);
+    return (tok - tok0) * qrow + h * (uint32_t)(a.qs[1] * 2) + (uint32_t)((lane % RPL) ^ (r & (RPL - 1))) * 16;
+  };
+  // loads [i0, i1) of it
+  auto load_q = [&](const Tile& t, int i0, int i1) {
+    const uint32_t tok0 = single ? (uint32_t)(t.w.it.tile * PW_ROWS)
+                                 : (uint32_t)(t.w.it.tile * PW_ROWS) / (uint32_t)a.group;
+    const uint8_t* p = a.q + (((int64_t)t.w.it.row0 + tok0) * a.qs[0] + (int64_t)t.hk * a.group * a.qs[1]) * 2;
+    const i32x4_t r = rsrc_words(p, 0xffffffffu);
+    if (single && (t.w.it.tile + 1) * PW_ROWS <= t.w.it.rows) {
+      // chunk (lane % RPL) ^ (row % RPL): the row's part of it below RPI is the lane's, above i's
+      const uint32_t off = (uint32_t)(wave * 64 + lane / RPL) * qrow;
+#pragma unroll 4
+      for (int i = i0; i < i1; ++i)
+        dma16s(r, qlds + i * 1024,
+               off + (uint32_t)((lane % RPL) ^ ((i * RPI + lane / RPL) & (RPL - 1))) * 16,
+               (uint32_t)(i * RPI) * qrow);
+    } else {
+#pragma unroll 1
+      for (int i = i0; i < i1; ++i)
+        dma16(r, lds + __builtin_amdgcn_readfirstlane((int)(qlds - lds) + i * 1024), q_offset(t, i, tok0));
+    }
+  };
+  // this wavefront's loads of a tile of K or V: slot (wave + 4 i) * 64 + lane of SLOTS a row is a row
+  // and a chunk of it, at the same offsets for every whole tile. Rows past the last key read that
+  // key again
+  auto key_offset = [&](int i, int slots, uint32_t row, int n) {
+    const int sl = (wave + 4 * i) * 64 + lane;
+    return (uint32_t)min(sl / slots, n - 1) * row + (uint32_t)min(sl % slots, RPL - 1) * 16;
+  };
+  uint32_t ko[(L::KS + 3) / 4], vo[(L::VS + 3) / 4];
+#pragma unroll
+  for (int i = 0; i < (L::KS + 3) / 4; ++i) ko[i] = key_offset(i, L::KS, (uint32_t)(a.ks[0] * 2), 64);
+#pragma unroll
+  for (int i = 0; i < (L::VS + 3) / 4; ++i) vo[i] = key_offset(i, L::VS, (uint32_t)(a.vs[0] * 2), 64);
+  auto load_keys = [&](const Tile& t, const uint8_t* base, const int64_t (&st)[2], int j, uint8_t* dst,
+                       const auto& off, auto slots) {
+    constexpr int S = decltype(slots)::value;
+    if (j >= t.nt) return;
+    const int n = min(t.w.keys - j * 64, 64);
+    const uint32_t row = (uint32_t)(st[0] * 2);
+    const uint8_t* p = base + (((int64_t)t.w.kbeg + j * 64) * st[0] + t.hk * st[1]) * 2;
+    const i32x4_t r = rsrc_words(p, (uint32_t)(n - 1) * row + D * 2);
+    if (n == 64) {
+#pragma unroll
+      for (int i = 0; i < (S + 3) / 4; ++i)
+        if (wave + 4 * i < S) dma16(r, dst + (wave + 4 * i) * 1024, off[i]);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < (S + 3) / 4; ++i)
+        if (wave + 4 * i < S)
+          dma16(r, lds + __builtin_amdgcn_readfirstlane((int)(dst - lds) + (wave + 4 * i) * 1024),
+                key_offset(i, S, row, n));
+    }
+  };
+  auto load_k = [&](const Tile& t, int j, int b) {
+    load_keys(t, a.k, a.ks, j, kbuf(b), ko, std::integral_constant<int, L::KS>{});
+  };
+  auto load_v = [&](const Tile& t, int j, int b) {
+    load_keys(t, a.v, a.vs, j, vbuf(b), vo, std::integral_constant<int, L::VS>{});
+  };
+
+  // a round of the launch's workgroups takes consecutive (key head, tile) pairs, those of an XCD
+  // consecutive ones among them: neighbours read the same keys through one L2
+  const int per = gridDim.x >> 3;
+  int64_t id = (gridDim.x & 7) == 0 ? (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
+  Tile t = find(id);
+  bool first = true;
+  if (t.w.it.req < 0) return;
+  int kb = 0;  // K(j) and V(j) of this row tile are in slots (kb + j) % 2
+  load_k(t, 0, 0);
+  load_q(t, 0, L::QL);
+  load_k(t, 1, 1), load_v(t, 0, 0);
+  for (;;) {
+    id += gridDim.x;
+    const Tile next = find(id);
+    const int nt = t.nt, keys = t.w.keys;
+    frag qf[2][NC];
+    f32x16 acc[2][NDT];
+    float m_run[2], l_run[2];
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+      m_run[gr] = 0.f, l_run[gr] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NDT; ++i) acc[gr][i] = f32x16{};
+    }
+    // V^T fragments: lane l of a 16-lane group supplies key row 4 g + (l / 4) % 4 of 8 keys and 4
+    // channels; it receives channel l % 32 of keys {4g .. 4g + 3} and {8 + 4g .. 8 + 4g + 3}
+    const uint32_t vl = (uint32_t)((4 * g + ((lane >> 2) & 3)) * (L::VS * 16) +
+                                   32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+    auto v_frag = [&](const uint8_t* sv, int half, int f) {
+      const int hh = f / NDT, dt = f % NDT;
+      const uint8_t* p = sv + vl + (half * 32 + hh * 16) * (L::VS * 16) + dt * 64;
+      const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)p);
+      const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(p + 8 * (L::VS * 16)));
+      const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+      return __builtin_bit_cast(frag, u32x4{l2[0], l2[1], h2[0], h2[1]});
+    };
+    auto k_frag = [&](const uint8_t* sk, int half, int c) {
+      return *reinterpret_cast<const frag*>(sk + (half * 32 + col) * (L::KS * 16) + (2 * c + g) * 16);
+    };
+    auto p_frag = [](const uint32_t (&pp)[8], int hh) {
+      return __builtin_bit_cast(frag, u32x4{pp[hh * 4], pp[hh * 4 + 1], pp[hh * 4 + 2], pp[hh * 4 + 3]});
+    };
+    const float cmul = a.scale_log2;
+    // One half h: exponentials of its scores `sc` into `pc` beside, with QK, the scores of half h + 1
+    // (half kh of the keys in sk) into `sn` and, with PV, the second product of half h - 1 (`pl`, half
+    // vh of the values in sv).
+    auto half_step = [&](auto qk, auto pv, f32x16 (&sc)[2], f32x16 (&sn)[2], uint32_t (&pl)[2][8],
+                         uint32_t (&pc)[2][8], const uint8_t* sk, int kh, const uint8_t* sv, int vh,
+                         int left) {
+      constexpr bool QK = decltype(qk)::value, PV = decltype(pv)::value;
+      if (left < 32) {  // keys past the request's last do not exist
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if ((v >> 2) * 8 + g * 4 + (v & 3) >= left) sc[gr][v] = -INFINITY;
+      }
+      if constexpr (!PV) {  // the first half: the reference is its maximum
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+          float mx = sc[gr][0];
+#pragma unroll
+          for (int v = 1; v < 16; ++v) mx = fmaxf(mx, sc[gr][v]);
+          m_run[gr] = fmaxf(pair_max(mx) * cmul, -FLT_MAX);
+        }
+      }
+      frag kf[3], vf[3];
+      auto read = [&](int c) {
+        if constexpr (QK) kf[c % 3] = k_frag(sk, kh, c);
+        if constexpr (PV) vf[c % 3] = v_frag(sv, vh, c);
+      };
+      float ls[2] = {0.f, 0.f};
+      auto exps = [&](int gr, int e) {  // pair e of group gr
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[gr][2 * e], cmul, -m_run[gr]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[gr][2 * e + 1], cmul, -m_run[gr]));
+        ls[gr] += p0 + p1;
+        pc[gr][e] = MfmaT<T>::pack2(p0, p1);
+        asm volatile("" : "+v"(pc[gr][e]));  // here, not where it is first read
+      };
+      constexpr int PER = 8 / NC;  // pairs a group of MFMAs: NC groups of two or four
+      read(0);
+      read(1);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (c + 2 < NC) read(c + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (QK)
+          sn[0] = MfmaT<T>::mma(kf[c % 3], qf[0][c], c == 0 ? f32x16{} : sn[0]);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) exps(0, c * PER + e);
+        if constexpr (QK) sn[1] = MfmaT<T>::mma(kf[c % 3], qf[1][c], c == 0 ? f32x16{} : sn[1]);
+        if constexpr (PV)
+          acc[0][c % NDT] = MfmaT<T>::mma(vf[c % 3], p_frag(pl[0], c / NDT), acc[0][c % NDT]);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) exps(1, c * PER + e);
+        if constexpr (PV)
+          acc[1][c % NDT] = MfmaT<T>::mma(vf[c % 3], p_frag(pl[1], c / NDT), acc[1][c % NDT]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (PV && __any(!(ls[0] < MfmaT<T>::kLazyLimit) || !(ls[1] < MfmaT<T>::kLazyLimit))) {
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[gr][v]);
+          const float m_use = fmaxf(m_run[gr], pair_max(mx) * cmul);
+          const float alpha = __builtin_amdgcn_exp2f(m_run[gr] - m_use);
+          m_run[gr] = m_use;
+          l_run[gr] *= alpha;
+#pragma unroll
+          for (int i = 0; i < NDT; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[gr][i][v] *= alpha;
+          ls[gr] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[gr][2 * e], cmul, -m_use));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[gr][2 * e + 1], cmul, -m_use));
+            ls[gr] += p0 + p1;
+            pc[gr][e] = MfmaT<T>::pack2(p0, p1);
+          }
+        }
+      }
+      l_run[0] += ls[0];
+      l_run[1] += ls[1];
+      // the accumulators stay where the matrix core has them: left free, they move out and back
+      // beside every half for the sake of the rescaling above, which hardly ever runs
+      if constexpr (PV)
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+          for (int i = 0; i < NDT; ++i) asm volatile("" : "+a"(acc[gr][i]));
+    };
+    auto last_pv = [&](uint32_t (&pl)[2][8], const uint8_t* sv, int vh) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const frag vf = v_frag(sv, vh, c);
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+          acc[gr][c % NDT] = MfmaT<T>::mma(vf, p_frag(pl[gr], c / NDT), acc[gr][c % NDT]);
+      }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    // K(0) and Q, loaded under the row tile before, have landed for every wavefront. Its output's
+    // stores, as many on every path, are younger and may be on their way, and between the two the
+    // loads of K(1) and V(0), where there are both
+    if (first) wide_barrier();
+    else if (nt > 1) wide_barrier<L::STORES + L::KS / 4 + L::VS / 4>();
+    else wide_barrier<L::STORES>();
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int r = gr * 32 + col;
+        u32x4 v = *reinterpret_cast<const u32x4*>(qlds + r * D * 2 + (((2 * c + g) ^ (r & (RPL - 1))) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] ^= a.q_sign;
+        qf[gr][c] = __builtin_bit_cast(frag, v);
+      }
+    int quarters = 0;  // of the next tile's Q on the way
+    auto load_quarter = [&]() {
+      if (next.w.it.req >= 0 && quarters < 4) {
+        load_q(next, quarters * L::QQ, (quarters + 1) * L::QQ);
+        ++quarters;
+        return true;
+      }
+      return false;
+    };
+    if (nt > 0) {
+      f32x16 sa[2], sb[2];
+      uint32_t pa[2][8], pb[2][8];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const frag kf = k_frag(kbuf(kb), 0, c);
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+          sa[gr] = MfmaT<T>::mma(kf, qf[gr][c], c == 0 ? f32x16{} : sa[gr]);
+      }
+      half_step(Yes{}, No{}, sa, sb, pb, pa, kbuf(kb), 1, nullptr, 0, keys);
+      // before half 2j - 1: K(j) and V(j - 1) have landed. For j = 1 only the stores are younger, after
+      // that a quarter of Q, if one was left to load
+      bool q_last = false;
+      auto landed = [&](int j) {
+        if (j == 1 && !first) wide_barrier<L::STORES>();
+        else if (q_last) wide_barrier<L::QQ>();
+        else wide_barrier();
+      };
+      for (int j = 1; j < nt; ++j) {
+        landed(j);
+        if (j + 1 < nt) load_k(t, j + 1, (kb + j + 1) & 1);
+        else if (next.w.it.req >= 0) load_k(next, 0, (kb + nt) & 1);
+        load_v(t, j, (kb + j) & 1);
+        q_last = load_quarter();
+        half_step(Yes{}, Yes{}, sb, sa, pa, pb, kbuf((kb + j) & 1), 0, vbuf((kb + j - 1) & 1), 0,
+                  keys - j * 64 + 32);
+        half_step(Yes{}, Yes{}, sa, sb, pb, pa, kbuf((kb + j) & 1), 1, vbuf((kb + j - 1) & 1), 1,
+                  keys - j * 64);
+      }
+      landed(nt);
+      if (next.w.it.req >= 0) {
+        if (nt == 1) load_k(next, 0, (kb + 1) & 1);
+        while (load_quarter()) {
+        }
+        load_k(next, 1, (kb + nt + 1) & 1), load_v(next, 0, (kb + nt) & 1);
+      }
+      const uint8_t* sv = vbuf((kb + nt - 1) & 1);
+      half_step(No{}, Yes{}, sb, sa, pa, pb, nullptr, 0, sv, 0, keys - nt * 64 + 32);
+      last_pv(pb, sv, 1);
+    } else if (next.w.it.req >= 0) {
+      __syncthreads();  // every wavefront has its rows of Q
+      load_k(next, 0, kb);
+      while (load_quarter()) {
+      }
+      load_k(next, 1, (kb + 1) & 1), load_v(next, 0, kb);
+    }
+    first = false;
+    // ---- normalize; lane: rows col of each group, channels dt * 32 + (v / 4) * 8 + 4 g + v % 4. 32 rows
+    // of 64 channels at a time go through 4 KB of the wavefront's own (chunk c of row r at c ^ (r % 8))
+    // and out as 128 bytes of a row by 8 lanes; a row that is not there is stored past the buffer's end
+    const uint32_t tok0 = single ? (uint32_t)(t.w.it.tile * PW_ROWS)
+                                 : (uint32_t)(t.w.it.tile * PW_ROWS) / (uint32_t)a.group;
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc(
+        a.o + (((int64_t)t.w.it.row0 + tok0) * a.os[0] + (int64_t)t.hk * a.group * a.os[1]) * 2, 0x80000000u);
+    uint8_t* olds = lds + 2 * (L::KB + L::VB) + 4 * L::QB + wave * 4096;
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+      const float l = pair_sum(l_run[gr]);
+      const float inv = keys == 0 ? 0.f : 1.0f / l;  // no keys: zeros
+      uint32_t off[4];  // of rows lane / 8 + 8 i
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t h;
+        const uint32_t tok = conv_udiv((uint32_t)(t.w.it.tile * PW_ROWS + wave * 64 + gr * 32 + i * 8 + lane / 8),
+                                       (uint32_t)a.group, a.group_m, h);
+        off[i] = tok < (uint32_t)t.w.it.rows ? (tok - tok0) * (uint32_t)(a.os[0] * 2) +
+                                                   h * (uint32_t)(a.os[1] * 2) + (lane & 7) * 16
+                                             : 0x80000000u;
+      }
+#pragma unroll
+      for (int d2 = 0; d2 < NDT; d2 += 2) {
+#pragma unroll
+        for (int dt = d2; dt < d2 + 2; ++dt)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<u32x2*>(olds + col * 128 + ((((dt - d2) * 4 + u) ^ (col & 7)) << 4) + g * 8) =
+                u32x2{MfmaT<T>::pack2(acc[gr][dt][4 * u] * inv, acc[gr][dt][4 * u + 1] * inv),
+                      MfmaT<T>::pack2(acc[gr][dt][4 * u + 2] * inv, acc[gr][dt][4 * u + 3] * inv)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + lane / 8;
+          const u32x4 w = *reinterpret_cast<const u32x4*>(olds + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          __builtin_amdgcn_raw_buffer_store_b128(w, ro, off[i] + d2 * 64, 0, 0);
+        }
+      }
+    }
+    if (next.w.it.req < 0) return;
+    kb = (kb + nt) & 1;
+    t = next;
   }
 }
 
@@ -523,16 +960,23 @@ struct PackedPlan {
   int64_t slots;        // chunks, at most
 };
 static PackedPlan packed_plan(int64_t rows_q, int64_t rows_k, int64_t requests, int64_t kv_heads,
-                              int64_t group) {
+                              int64_t group, bool wide_strides) {
   PackedPlan p = {};
   // tiles of 32 rows where requests have fewer than 48 on average
   const bool few = rows_q * group <= 48 * std::max<int64_t>(requests, 1);
-  p.block = few ? PF_ROWS : PA_ROWS;
+  // tiles of 256 where requests fill them and every compute unit has two (us, tiles of 256 against
+  // 128; 24 heads of 128 channels unless said): 264 tiles to 512 keys 54 to 48, 528 tiles 72 to 71
+  // (64 keys: 27.6 to 33.7), 792 tiles to 256 keys 61 to 66, 40 heads 2560 tiles to 512 keys 232 to
+  // 280; 60 requests of 83 rows 103 to 66, of 200 rows 71 to 74
+  const bool wide = !few && wide_strides && requests <= PACKED_LANES &&
+                    rows_q * group >= PW_ROWS * requests &&
+                    (rows_q * group / PW_ROWS) * kv_heads >= 512;
+  p.block = few ? PF_ROWS : wide ? PW_ROWS : PA_ROWS;
   p.key_tile = few ? PF_KEYS : PA_KEYS;
   p.items = (int)((rows_q * group + p.block - 1) / p.block + requests + 2);
   // two workgroups for each compute unit; launches of as many row tiles keep their keys whole
   constexpr int kGroups = 512;
-  if (requests > 0 && requests <= PACKED_LANES && rows_k > p.key_tile &&
+  if (!wide && requests > 0 && requests <= PACKED_LANES && rows_k > p.key_tile &&
       p.items * kv_heads < kGroups) {
     p.groups = kGroups;
     // PackedChunks::scan's count: at most `groups` and one for every row tile (and a few, for the
@@ -559,7 +1003,7 @@ extern "C" int64_t difflet_rocm_packed_attention_workspace_bytes(int64_t rows_q,
   if (rows_q <= 0 || rows_k <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 ||
       kv_heads * group > 65536 || rows_q * group >= (1LL << 30) || requests >= (1LL << 24))
     return 0;
-  return packed_workspace(packed_plan(rows_q, rows_k, requests, kv_heads, group), head_dim);
+  return packed_workspace(packed_plan(rows_q, rows_k, requests, kv_heads, group, true), head_dim);
 }
 
 extern "C" int difflet_rocm_packed_attention(
@@ -616,7 +1060,14 @@ extern "C" int difflet_rocm_packed_attention(
   // weighs any real score as 0 does
   a.scale_log2 = std::max((scale < 0 ? -scale : scale) * LOG2E, FLT_MIN);
   a.q_sign = scale < 0 ? 0x80008000u : 0u;
-  const PackedPlan plan = packed_plan(rows_q, rows_k, requests, kv_heads, group);
+  // the wide kernel addresses a tile's rows of q and o in 31 bits and stores 16 bytes of o
+  auto near = [&](const int64_t* st) {
+    return st[0] >= 0 && st[1] >= 0 && st[0] < (1LL << 29) && st[1] < (1LL << 29) &&
+           (PW_ROWS / group + 2) * st[0] + group * st[1] + head_dim < (1LL << 29);
+  };
+  const bool wide_strides = near(q_strides) && near(o_strides) && ((uintptr_t)o & 15) == 0 &&
+                            o_strides[0] % 8 == 0 && o_strides[1] % 8 == 0;
+  const PackedPlan plan = packed_plan(rows_q, rows_k, requests, kv_heads, group, wide_strides);
   a.items = plan.items;
   if (plan.groups && workspace && workspace_bytes >= packed_workspace(plan, head_dim)) {
     DLT_REQUIRE(((uintptr_t)workspace & 255) == 0, DIFFLET_EINVAL,
@@ -626,6 +1077,7 @@ extern "C" int difflet_rocm_packed_attention(
     a.stats = (f32x2*)workspace;
     a.part = (float*)((uint8_t*)workspace + packed_stats_bytes(plan));
   }
+  a.group_m = conv_magic((uint32_t)group);
   const int64_t blocks = a.groups ? a.groups : (int64_t)a.items * kv_heads;
   DLT_REQUIRE(blocks < (1LL << 31), DIFFLET_EUNSUPPORTED, "%s: too many tiles", name);
   hipStream_t s = (hipStream_t)stream;
@@ -634,6 +1086,12 @@ extern "C" int difflet_rocm_packed_attention(
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
     const bool few = plan.block == PF_ROWS;
+    if (plan.block == PW_ROWS) {
+      // one workgroup a compute unit
+      const dim3 cus((unsigned)std::min<int64_t>(blocks, std::max(gemm_device_cus(), 1)));
+      hipLaunchKernelGGL((packed_attn_wide_kernel<T, D>), cus, block, 0, s, a);
+      return;
+    }
     if (!a.groups) {
       if (few) hipLaunchKernelGGL((packed_attn_few_kernel<T, D, false>), grid, block, 0, s, a);
       else hipLaunchKernelGGL((packed_attn_kernel<T, D, false>), grid, block, 0, s, a);

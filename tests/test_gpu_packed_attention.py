@@ -227,3 +227,107 @@ def test_packed_cross_attention_compiles(gpu):
                       fullgraph=True, backend="aot_eager")
     want = packed_cross_attention(q * 2, k, v, qs, ks, scale=0.1) + 1
     assert torch.equal(f(q, k, v), want)
+
+
+MANY = [
+    ([9000, 7100], [100, 513], 16, 16, 128), ([12000, 1, 0, 300, 4000], [64, 65, 7, 0, 31], 16, 16, 128),
+    ([3333], [1200], 70, 10, 128), ([39000, 700, 26001], [32, 96, 0], 2, 2, 64),
+    ([4000, 8100], [77, 300], 24, 12, 64), ([131073], [1], 1, 1, 128), ([300] * 62, [29] * 62, 8, 8, 128),
+    ([300] * 63, [29] * 63, 8, 8, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,keys,h,hk,d", MANY)
+def test_packed_cross_attention_of_many_rows(gpu, lengths, keys, h, hk, d, dtype):
+    """Whole and ragged tiles of 256 rows, one to eight and more tiles of keys, requests without any,
+    heads that share keys; more requests than a wavefront has lanes."""
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    q, k, v = case(gpu, dtype, lengths, keys, h, hk, d, seed=1)
+    got = packed_cross_attention(q, k, v, starts(lengths, gpu), starts(keys, gpu), scale=d ** -0.5)
+    check(got, exact(q, k, v, lengths, keys, d ** -0.5))
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_packed_cross_attention_of_many_rows_scales(gpu, scale):
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    lengths, keys = [9000, 8000], [200, 333]
+    q, k, v = case(gpu, BF16, lengths, keys, 16, 8, 64, std=0.5)
+    got = packed_cross_attention(q, k, v, starts(lengths, gpu), starts(keys, gpu), scale=scale)
+    check(got, exact(q, k, v, lengths, keys, scale))
+
+
+@pytest.mark.parametrize("offset", [4, 8])  # rows of the output on 8 or 16 bytes
+@pytest.mark.parametrize("h,hk", [(16, 16), (12, 4)])
+def test_packed_cross_attention_of_many_rows_strides_and_rows_of_no_request(gpu, h, hk, offset):
+    from difflet_amd import kernels
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    g = torch.Generator(device=gpu).manual_seed(5)
+    d, lengths, keys = 128, [9001, 600, 3000], [130, 0, 450]
+    rows, states = sum(lengths) + 12, sum(keys) + 9
+    buf = torch.randn(rows, 2 * h * d + 8, generator=g, device=gpu).to(BF16)
+    kv = torch.randn(states, 3 * hk * d, generator=g, device=gpu).to(BF16)
+    q = buf[:, h * d:2 * h * d].unflatten(-1, (h, d))
+    k, v = (kv[:, i * hk * d:(i + 1) * hk * d].unflatten(-1, (hk, d)) for i in (0, 2))
+    kv[:4] = float("inf")
+    kv[4 + sum(keys):] = float("nan")
+    q_starts, k_starts = starts(lengths, gpu, 5), starts(keys, gpu, 4)
+    want = exact(q, k, v, lengths, keys, d ** -0.5, 5, 4)
+    got = packed_cross_attention(q, k, v, q_starts, k_starts, scale=d ** -0.5)
+    check(got, want)
+    end = 5 + sum(lengths)
+    assert not bool(got[:5].any()) and not bool(got[end:].any())
+    out = torch.full((rows, h * d + 8), 7.0, dtype=BF16, device=gpu)
+    o = out[:, offset:offset + h * d].unflatten(-1, (h, d))
+    kernels.packed_attention(q, k, v, q_starts, k_starts, scale=d ** -0.5, out=o)
+    check(o[5:end], tuple(t[5:end] for t in want))
+    assert bool((out[:5] == 7).all()) and bool((out[end:] == 7).all())
+    assert bool((out[:, :offset] == 7).all()) and bool((out[:, offset + h * d:] == 7).all())
+
+
+def test_packed_cross_attention_of_many_rows_extremes(gpu):
+    """A NaN in one request's states, an infinity in another's values, scores that grow along the keys
+    by far more than the first keys' maximum: each stays in its request."""
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    lengths, keys = [9000, 8000, 300, 1100], [500, 600, 700, 900]
+    q, k, v = case(gpu, BF16, lengths, keys, 8, 8, 128)
+    qs, ks = starts(lengths, gpu), starts(keys, gpu)
+    k[500 + 600 + 700:] = k[500 + 600 + 700:] * torch.linspace(0.1, 30, 900, device=gpu).to(BF16)[:, None, None]
+    check(packed_cross_attention(q, k, v, qs, ks, scale=0.3), exact(q, k, v, lengths, keys, 0.3))
+    k[503, 0, 5] = float("nan")
+    v[1105, 1, 9] = float("inf")
+    got = packed_cross_attention(q, k, v, qs, ks, scale=0.001)
+    a, b, c = 9000, 17000, 17300
+    assert bool(got[:a].isfinite().all()) and bool(got[c:].isfinite().all())
+    assert bool(got[a:b, 0].isnan().all()) and bool(got[a:b, 1:].isfinite().all())
+    assert bool((got[b:c, 1, 9] == float("inf")).all()) and bool(got[b:c, 0].isfinite().all())
+
+
+def test_packed_cross_attention_of_many_rows_graph_follows_new_lengths(gpu):
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    rows, states = 17000, 1500
+    q, k, v = case(gpu, BF16, [rows], [states], 8, 8, 64)
+    qs, ks = starts([1, rows - 1], gpu), starts([1000, 500], gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        packed_cross_attention(q, k, v, qs, ks, scale=0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = packed_cross_attention(q, k, v, qs, ks, scale=0.1)
+    for i, (lengths, keys) in enumerate((([1, rows - 1], [1000, 500]), ([rows - 1, 1], [1500, 0]),
+                                         ([9000, 7000], [1, 1300]), ([0, rows], [64, 65]))):
+        qs.copy_(starts(lengths, gpu))
+        ks.copy_(starts(keys, gpu))
+        q.copy_(case(gpu, BF16, [rows], [states], 8, 8, 64, seed=i)[0])
+        graph.replay()
+        want = packed_cross_attention(q, k, v, qs, ks, scale=0.1)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        check(out, exact(q, k, v, lengths, keys, 0.1))
