@@ -269,7 +269,7 @@ extern "C" int difflet_rocm_lora_linear(int kind, const void* a, int64_t lda, co
     const dim3 g((unsigned)grid), b(256);
     if (lora_wide(m, requests)) {
       if (nr == 1) hipLaunchKernelGGL((lora_down_wide_kernel<1, 4>), g, b, 0, s, d);
-      else if (nr == 2) hipLaunchKernelGGL((lora_down_wide_kernel<2, 4>), g, b, 0, s, d);
+      else if (nr == 2) hipLaunchKernelGGL((lora_down_wide_kernel<2, 3>), g, b, 0, s, d);
       else hipLaunchKernelGGL((lora_down_wide_kernel<4, 4>), g, b, 0, s, d);
     } else if (nr == 1) {
       hipLaunchKernelGGL((lora_down_kernel<1>), g, b, 0, s, d);

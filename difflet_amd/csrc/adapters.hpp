@@ -48,6 +48,54 @@ __device__ __forceinline__ int lora_row_adapter(const LoraDev& L, int m, Start s
   return (uint32_t)a < (uint32_t)L.adapters ? a : -1;
 }
 
+// Whether rows [m0, end) of a tile are all of one request, or of none: their adapter, -1 for none, -2
+// for a tile that is not like that (or more requests than this looks at). load() reads what find()
+// needs, which a kernel does before its K loop, so that nothing of it is waited for behind.
+struct LoraOne {
+  static constexpr int MOST = kWave - 1;
+  int start = 0, id = -1;  // of request `lane`; lane `requests` the last row number
+  __device__ __forceinline__ void load(const LoraDev& L) {
+    const int lane = threadIdx.x & (kWave - 1);
+    if (L.requests == 0 || L.requests > MOST) return;
+    start = packed_start(L.starts, min(lane, L.requests), L.m);
+    id = L.ids[min(lane, L.requests - 1)];
+  }
+  __device__ __forceinline__ int find(const LoraDev& L, int m0, int end) const {
+    if (L.requests == 0) return -1;
+    if (L.requests > MOST) return -2;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int n = __popcll(__ballot(lane < L.requests && start <= m0));  // that start at or before m0
+    const int next = __builtin_amdgcn_readlane(start, n);  // n == requests: where the last one ends
+    if (n == L.requests && next <= m0) return -1;
+    if (next < end) return -2;
+    const int a = n ? __builtin_amdgcn_readlane(id, max(n - 1, 0)) : -1;
+    return (uint32_t)a < (uint32_t)L.adapters ? a : -1;
+  }
+};
+
+// Eight rank values at p, their pieces added in order, the loads of FLY pieces at a time in flight.
+template <int FLY>
+__device__ __forceinline__ void lora_v8(const LoraDev& L, const float* p, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll 1
+  for (int q = 0; q < L.pieces; q += FLY, p += FLY * L.v_piece) {
+    f32x4 t[FLY][2];
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) {
+      t[i][0] = t[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (q + i < L.pieces) {
+        t[i][0] = *reinterpret_cast<const f32x4*>(p + i * L.v_piece);
+        t[i][1] = *reinterpret_cast<const f32x4*>(p + i * L.v_piece + 4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FLY; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[i][e >> 2][e & 3];
+  }
+}
+
 // Slots of the tile's rows m0 .. m0 + BM - 1: slot[r] (-1 for rows without an adapter or past m),
 // list[s] the adapter of slot s; returns how many slots there are. bad: [slots][BN / 32] zeros and,
 // ahead of them, a zero flag. `book`: LDS that is free, by all NT >= BM threads; ends with a barrier.
@@ -125,79 +173,130 @@ __device__ __forceinline__ bool lora_finite8(u32x4& w) {
   return any;
 }
 
-// The further K stages of a BM x BN tile at (m0, n0): `stage` is LDS for (BM + BN) rows of 128
-// bytes in the GEMMs' layout (chunk c of row r at c ^ swz(r)), `book` as above, both free when this
-// is called by all NT threads after a barrier. mma(ks) runs K step ks (16 values) of the staged
-// operands into the accumulators; poison(slot, bad) makes those NaN whose row's slot s has bit n of
-// bad[s * BN / 32 ..] set for their column n.
-template <int BM, int BN, int NT, typename Swz, typename Mma, typename Poison>
-__device__ __forceinline__ void lora_stages(const LoraDev& L, int m0, int n0, uint8_t* stage,
-                                            uint8_t* book, Swz swz, Mma mma, Poison poison) {
-  int *slot, *list;
-  uint32_t* bad;
-  const int slots = lora_slots<BM, BN, NT>(L, m0, book, slot, list, bad);
-  const int per = L.ldv >> 3;  // chunks of 8 ranks of an adapter
-  const int total = slots * per;
+// Ranks r8 .. r8 + 7 (r8 < rank) of column n of adapter a, those past the rank zero.
+__device__ __forceinline__ u32x4 lora_up8(const LoraDev& L, int a, int n, int r8) {
+  const bf16* p = L.up + ((int64_t)a * L.n + n) * L.rank + r8;
+  if ((L.rank & 7) == 0) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 w = {0u, 0u, 0u, 0u};  // rows of B off 16 bytes
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (r8 + e < L.rank) w[e >> 1] |= (uint32_t)h[e] << (16 * (e & 1));
+  return w;
+}
+
+// Chunks c0 .. c0 + 7 of adapter a's ranks into LDS (c0 a multiple of 8, `per` chunks in all), for rows
+// that all have it: the rows' values and the columns' each lie in one piece of memory, which the
+// threads read end to end. Ends with a barrier.
+template <int BM, int BN, int NT, int FLY, typename Swz>
+__device__ __forceinline__ void lora_stage_one(const LoraDev& L, int m0, int n0, int a, int c0, int per,
+                                               uint8_t* stage, Swz swz) {
+  const int tid = threadIdx.x;
+  const int n8 = min(per - c0, 8), pairs = (n8 + 1) & ~1;  // K steps take two chunks
+  const uint32_t inv = 65535u / (uint32_t)pairs + 1;       // i / pairs, exact below 2048
+  constexpr int PX = BM * 8 / NT, PW = BN * 8 / NT;
+  u32x4 x[PX], w[PW];
+#pragma unroll
+  for (int k = 0; k < PW; ++k) {
+    const int i = k * NT + tid, r = (int)((uint32_t)i * inv >> 16), ch = i - r * pairs;
+    w[k] = u32x4{0u, 0u, 0u, 0u};
+    if (r < BN && n0 + r < L.n && ch < n8 && (c0 + ch) * 8 < L.rank)
+      w[k] = lora_up8(L, a, n0 + r, (c0 + ch) * 8);
+  }
+#pragma unroll
+  for (int k = 0; k < PX; ++k) {
+    const int i = k * NT + tid, r = (int)((uint32_t)i * inv >> 16), ch = i - r * pairs;
+    float v[8] = {};
+    if (r < BM && m0 + r < L.m && ch < n8)
+      lora_v8<FLY>(L, L.v + (int64_t)(m0 + r) * L.ldv + (c0 + ch) * 8, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[k][e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+  }
+#pragma unroll
+  for (int k = 0; k < PX; ++k) {
+    const int i = k * NT + tid, r = (int)((uint32_t)i * inv >> 16), ch = i - r * pairs;
+    if (r < BM) *reinterpret_cast<u32x4*>(stage + r * 128 + ((ch ^ swz(r)) << 4)) = x[k];
+  }
+#pragma unroll
+  for (int k = 0; k < PW; ++k) {
+    const int i = k * NT + tid, r = (int)((uint32_t)i * inv >> 16), ch = i - r * pairs;
+    if (r < BN) *reinterpret_cast<u32x4*>(stage + (BM + r) * 128 + ((ch ^ swz(r)) << 4)) = w[k];
+  }
+  __syncthreads();
+}
+
+// Chunks c0 .. c0 + 7 of the slots' ranks into LDS (c0 a multiple of 8): the rows' rank values and the
+// adapters' columns. Ends with a barrier.
+template <int BM, int BN, int NT, int FLY, typename Swz>
+__device__ __forceinline__ void lora_stage(const LoraDev& L, int m0, int n0, int c0, int total, int per,
+                                           const int* slot, const int* list, uint32_t* bad,
+                                           uint8_t* stage, Swz swz) {
   const int tid = threadIdx.x, ch = tid & 7;
   constexpr int RP = NT / 8;  // rows a pass
+  const int vc = c0 + ch, s = vc / per, r8 = (vc - s * per) * 8;
+  const bool on = vc < total;
+  const int a = on ? list[s] : 0;
+  u32x4 w[BN / RP];
+#pragma unroll
+  for (int i = 0; i < BN / RP; ++i) {
+    const int n = n0 + i * RP + (tid >> 3);
+    w[i] = u32x4{0u, 0u, 0u, 0u};
+    if (!on || n >= L.n || r8 >= L.rank) continue;
+    w[i] = lora_up8(L, a, n, r8);
+    if (lora_finite8(w[i])) {
+      const int c = n - n0;
+      atomicOr(&bad[s * (BN / 32) + (c >> 5)], 1u << (c & 31));
+      bad[-1] = 1u;
+    }
+  }
+  u32x4 x[BM / RP];
+#pragma unroll
+  for (int i = 0; i < BM / RP; ++i) {
+    const int r = i * RP + (tid >> 3);
+    float v[8] = {};
+    if (on && slot[r] == s) lora_v8<FLY>(L, L.v + (int64_t)(m0 + r) * L.ldv + r8, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < BM / RP; ++i) {
+    const int r = i * RP + (tid >> 3);
+    *reinterpret_cast<u32x4*>(stage + r * 128 + ((ch ^ swz(r)) << 4)) = x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < BN / RP; ++i) {
+    const int r = i * RP + (tid >> 3);
+    *reinterpret_cast<u32x4*>(stage + (BM + r) * 128 + ((ch ^ swz(r)) << 4)) = w[i];
+  }
+  __syncthreads();
+}
+
+// The further K stages of a BM x BN tile at (m0, n0), whose rows all have adapter `one`, or, below 0,
+// not. `stage` is LDS for (BM + BN) rows of 128 bytes in the GEMMs' layout (chunk c of row r at c ^
+// swz(r)), `book` as above, both idle once every wavefront is here. mma(ks) runs K step ks (16
+// values) of the staged operands into the accumulators; poison(slot, bad) makes those NaN whose row's
+// slot s has bit n of bad[s * BN / 32 ..] set for their column n. Called by all NT threads.
+template <int BM, int BN, int NT, int FLY, typename Swz, typename Mma, typename Poison>
+__device__ __forceinline__ void lora_stages(const LoraDev& L, int m0, int n0, int one, uint8_t* stage,
+                                            uint8_t* book, Swz swz, Mma mma, Poison poison) {
+  int *slot = nullptr, *list = nullptr;
+  uint32_t* bad = nullptr;
+  const bool many = one < 0;
+  int slots = 1;
+  __syncthreads();  // every wavefront's reads of the ring are done
+  if (many) slots = lora_slots<BM, BN, NT>(L, m0, book, slot, list, bad);
+  const int per = L.ldv >> 3;  // chunks of 8 ranks of an adapter
+  const int total = slots * per;
+#pragma unroll 1
   for (int c0 = 0; c0 < total; c0 += 8) {
-    const int vc = c0 + ch, s = vc / per, r8 = (vc - s * per) * 8;
-    const bool on = vc < total;
-    const int a = on ? list[s] : 0;
-    u32x4 w[BN / RP];
-#pragma unroll
-    for (int i = 0; i < BN / RP; ++i) {
-      const int n = n0 + i * RP + (tid >> 3);
-      w[i] = u32x4{0u, 0u, 0u, 0u};
-      if (!on || n >= L.n || r8 >= L.rank) continue;
-      const bf16* p = L.up + ((int64_t)a * L.n + n) * L.rank + r8;
-      if ((L.rank & 7) == 0) {
-        w[i] = *reinterpret_cast<const u32x4*>(p);
-      } else {  // rows of B off 16 bytes
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (r8 + e < L.rank) w[i][e >> 1] |= (uint32_t)h[e] << (16 * (e & 1));
-      }
-      if (lora_finite8(w[i])) {
-        const int c = n - n0;
-        atomicOr(&bad[s * (BN / 32) + (c >> 5)], 1u << (c & 31));
-        bad[-1] = 1u;
-      }
-    }
-    u32x4 x[BM / RP];
-#pragma unroll
-    for (int i = 0; i < BM / RP; ++i) {
-      const int r = i * RP + (tid >> 3);
-      float v[8] = {};
-      if (on && slot[r] == s) {
-        const float* p = L.v + (int64_t)(m0 + r) * L.ldv + r8;
-        for (int q = 0; q < L.pieces; ++q, p += L.v_piece) {
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(p);
-          const f32x4 hi = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[i][e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-    }
-#pragma unroll
-    for (int i = 0; i < BM / RP; ++i) {
-      const int r = i * RP + (tid >> 3);
-      *reinterpret_cast<u32x4*>(stage + r * 128 + ((ch ^ swz(r)) << 4)) = x[i];
-    }
-#pragma unroll
-    for (int i = 0; i < BN / RP; ++i) {
-      const int r = i * RP + (tid >> 3);
-      *reinterpret_cast<u32x4*>(stage + (BM + r) * 128 + ((ch ^ swz(r)) << 4)) = w[i];
-    }
-    __syncthreads();
+    if (many) lora_stage<BM, BN, NT, FLY>(L, m0, n0, c0, total, per, slot, list, bad, stage, swz);
+    else lora_stage_one<BM, BN, NT, FLY>(L, m0, n0, one, c0, per, stage, swz);
     const int steps = (min(total - c0, 8) + 1) >> 1;
+#pragma unroll 1
     for (int ks = 0; ks < steps; ++ks) mma(ks);
     __syncthreads();
   }
-  if (total > 0 && bad[-1]) poison(slot, bad);
+  if (many && total > 0 && bad[-1]) poison(slot, bad);
 }
 
 }  // namespace dlt

@@ -358,6 +358,10 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
   const int frow = lane & 31;  // fragment row within a 32-row MFMA tile
   const int fhalf = lane >> 5;
 
+  [[maybe_unused]] LoraOne lora_rows;
+  [[maybe_unused]] int lora_one = -2;
+  if constexpr (LORA) lora_rows.load(args.lora);
+
   static_assert(KTB == 128 && NSLOT == 2, "the K loop runs 128-byte stages in two slots");
   {
     // ---- 128-byte stages in two LDS slots. A stage is NKS MFMA K steps (bf16 4 of 16 elements,
@@ -443,6 +447,7 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
       __builtin_amdgcn_s_waitcnt(0x0f70);
     }
     __syncthreads();
+    if constexpr (LORA) lora_one = lora_rows.find(args.lora, (int)m0, min((int)m0 + BM, M));
     read_w(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) read_a(0, 0, 0, i);
@@ -475,7 +480,6 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
   }
 
   if constexpr (LORA) {
-    __syncthreads();  // every wave's last fragment reads of the ring are done
     if constexpr (E == Elem::FP8) {
       float sa[4];
 #pragma unroll
@@ -497,9 +501,10 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
             for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= sa[i] * wv[e];
         }
     }
-    if (kbeg == 0)
-      lora_stages<BM, BN, 128 * WN>(
-          args.lora, (int)m0, (int)n0, lds, lds + (BM + BN) * KTB, [](int r) { return swz8(r); },
+    if (kbeg == 0 && lora_one != -1)
+      lora_stages<BM, BN, 128 * WN, 1>(
+          args.lora, (int)m0, (int)n0, lora_one, lds,
+          lds + (BM + BN) * KTB, [](int r) { return swz8(r); },
           [&](int ks) {
             bf16x8 fx[4], fy[4];
 #pragma unroll

@@ -312,6 +312,13 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
       }
   };
 
+  // before the untracked loads: the compiler waits for all of those with its own
+  [[maybe_unused]] int lora_one = -2;
+  if constexpr (LORA) {
+    LoraOne rows;
+    rows.load(args.lora);
+    lora_one = rows.find(args.lora, m0, m0 + arows);
+  }
   issue_scales(0);
   issue_scales(1);
 #pragma unroll
@@ -381,9 +388,10 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
             for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= sa[i] * wv[e];
         }
     }
-    if (piece == 0)
-      lora_stages<BM, BN, NT>(
-          args.lora, m0, n0, lds, lds + SLOT, [](int r) { return swz8s(r); },
+    if (piece == 0 && lora_one != -1) {
+      lora_stages<BM, BN, NT, 8>(
+          args.lora, m0, n0, lora_one, lds, lds + SLOT,
+          [](int r) { return swz8s(r); },
           [&](int ks) {
             bf16x8 fx[4], fy[4];
             auto at = [&](int r) { return r * 128 + (((2 * ks + fhalf) ^ swz8s(r)) << 4); };
@@ -413,7 +421,8 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
               }
             }
           });
-    __syncthreads();
+      __syncthreads();
+    }
   }
   float* tile = reinterpret_cast<float*>(lds);
   constexpr int CM = BN / 4 < 32 ? BN / 4 - 1 : 31;
