@@ -71,6 +71,13 @@ struct LoraOne {
     const int a = n ? __builtin_amdgcn_readlane(id, max(n - 1, 0)) : -1;
     return (uint32_t)a < (uint32_t)L.adapters ? a : -1;
   }
+  // The adapter of row m (-1: none), of each lane's own, by all lanes; at most MOST requests.
+  __device__ __forceinline__ int of_row(const LoraDev& L, int m) const {
+    int n = 0;
+    for (int i = 0; i < L.requests; ++i) n += __builtin_amdgcn_readlane(start, i) <= m;
+    const int end = __shfl(start, n, kWave), a = __shfl(id, max(n - 1, 0), kWave);
+    return n && m < end && (uint32_t)a < (uint32_t)L.adapters ? a : -1;
+  }
 };
 
 // Eight rank values at p, their pieces added in order, the loads of FLY pieces at a time in flight.
@@ -99,9 +106,10 @@ __device__ __forceinline__ void lora_v8(const LoraDev& L, const float* p, float 
 // Slots of the tile's rows m0 .. m0 + BM - 1: slot[r] (-1 for rows without an adapter or past m),
 // list[s] the adapter of slot s; returns how many slots there are. bad: [slots][BN / 32] zeros and,
 // ahead of them, a zero flag. `book`: LDS that is free, by all NT >= BM threads; ends with a barrier.
+// Up to LoraOne::MOST requests are in the lanes' registers already (`rows`).
 template <int BM, int BN, int NT>
-__device__ __forceinline__ int lora_slots(const LoraDev& L, int m0, uint8_t* book, int*& slot,
-                                          int*& list, uint32_t*& bad) {
+__device__ __forceinline__ int lora_slots(const LoraDev& L, const LoraOne& rows, int m0, uint8_t* book,
+                                          int*& slot, int*& list, uint32_t*& bad) {
   static_assert(BM <= 256 && BM <= NT, "a thread per row");
   int* ints = reinterpret_cast<int*>(book);
   int *starts = ints, *ids = ints + LORA_LDS_REQUESTS + 1;
@@ -110,16 +118,18 @@ __device__ __forceinline__ int lora_slots(const LoraDev& L, int m0, uint8_t* boo
   int* count = list + 256;
   bad = reinterpret_cast<uint32_t*>(count + 2);
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  const bool in_lds = L.requests <= LORA_LDS_REQUESTS;
-  if (in_lds) {
+  const bool in_regs = L.requests <= LoraOne::MOST, in_lds = L.requests <= LORA_LDS_REQUESTS;
+  if (in_lds && !in_regs) {
     for (int i = tid; i <= L.requests; i += NT) starts[i] = packed_start(L.starts, i, L.m);
     for (int i = tid; i < L.requests; i += NT) ids[i] = L.ids[i];
+    __syncthreads();
   }
-  __syncthreads();
   if (tid < BM) {
     const int m = m0 + tid;
     int a = -1;
-    if (m < L.m) {
+    if (in_regs) {
+      a = rows.of_row(L, m);
+    } else if (m < L.m) {
       if (in_lds)
         a = lora_row_adapter(L, m, [&](int i) { return starts[i]; }, [&](int i) { return ids[i]; });
       else
@@ -132,20 +142,21 @@ __device__ __forceinline__ int lora_slots(const LoraDev& L, int m0, uint8_t* boo
   // one wavefront numbers the distinct adapters in the order of their first rows: a round per
   // adapter and 64 rows, and most tiles have one or two
   if (tid < kWave) {
-    int n = 0;
+    int n = 0, mine = -1;  // mine: list[lane], the first 64 of the list
     for (int c = 0; c < BM; c += kWave) {
       const int a = slot[c + lane];
       int s = -1;
       uint64_t left = __ballot(a >= 0);
       while (left) {
         const int b = __builtin_amdgcn_readlane(a, __ffsll((unsigned long long)left) - 1);
-        int at = -1;
-        for (int i = 0; i < n && at < 0; i += kWave) {
+        int at = __ffsll((unsigned long long)__ballot(mine == b)) - 1;
+        for (int i = kWave; i < n && at < 0; i += kWave) {
           const uint64_t hit = __ballot(i + lane < n && list[i + lane] == b);
           if (hit) at = i + __ffsll((unsigned long long)hit) - 1;
         }
         if (at < 0) {
           at = n++;
+          if (lane == at) mine = b;
           if (lane == 0) list[at] = b;
           __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         }
@@ -277,14 +288,15 @@ __device__ __forceinline__ void lora_stage(const LoraDev& L, int m0, int n0, int
 // values) of the staged operands into the accumulators; poison(slot, bad) makes those NaN whose row's
 // slot s has bit n of bad[s * BN / 32 ..] set for their column n. Called by all NT threads.
 template <int BM, int BN, int NT, int FLY, typename Swz, typename Mma, typename Poison>
-__device__ __forceinline__ void lora_stages(const LoraDev& L, int m0, int n0, int one, uint8_t* stage,
-                                            uint8_t* book, Swz swz, Mma mma, Poison poison) {
+__device__ __forceinline__ void lora_stages(const LoraDev& L, const LoraOne& rows, int m0, int n0,
+                                            int one, uint8_t* stage, uint8_t* book, Swz swz, Mma mma,
+                                            Poison poison) {
   int *slot = nullptr, *list = nullptr;
   uint32_t* bad = nullptr;
   const bool many = one < 0;
   int slots = 1;
   __syncthreads();  // every wavefront's reads of the ring are done
-  if (many) slots = lora_slots<BM, BN, NT>(L, m0, book, slot, list, bad);
+  if (many) slots = lora_slots<BM, BN, NT>(L, rows, m0, book, slot, list, bad);
   const int per = L.ldv >> 3;  // chunks of 8 ranks of an adapter
   const int total = slots * per;
 #pragma unroll 1

@@ -503,8 +503,8 @@ __global__ __launch_bounds__(128 * WN, 1) void gemm_kernel(
     }
     if (kbeg == 0 && lora_one != -1)
       lora_stages<BM, BN, 128 * WN, 1>(
-          args.lora, (int)m0, (int)n0, lora_one, lds,
-          lds + (BM + BN) * KTB, [](int r) { return swz8(r); },
+          args.lora, lora_rows, (int)m0, (int)n0, lora_one, lds, lds + (BM + BN) * KTB,
+          [](int r) { return swz8(r); },
           [&](int ks) {
             bf16x8 fx[4], fy[4];
 #pragma unroll

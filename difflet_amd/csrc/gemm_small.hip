@@ -313,11 +313,11 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
   };
 
   // before the untracked loads: the compiler waits for all of those with its own
+  [[maybe_unused]] LoraOne lora_rows;
   [[maybe_unused]] int lora_one = -2;
   if constexpr (LORA) {
-    LoraOne rows;
-    rows.load(args.lora);
-    lora_one = rows.find(args.lora, m0, m0 + arows);
+    lora_rows.load(args.lora);
+    lora_one = lora_rows.find(args.lora, m0, m0 + arows);
   }
   issue_scales(0);
   issue_scales(1);
@@ -389,9 +389,8 @@ __global__ __launch_bounds__(BN == 64 ? 256 : 512, 1) void gemm_small_kernel(
         }
     }
     if (piece == 0 && lora_one != -1) {
-      lora_stages<BM, BN, NT, 8>(
-          args.lora, m0, n0, lora_one, lds, lds + SLOT,
-          [](int r) { return swz8s(r); },
+      lora_stages<BM, BN, NT, BM == 64 ? 16 : 8>(
+          args.lora, lora_rows, m0, n0, lora_one, lds, lds + SLOT, [](int r) { return swz8s(r); },
           [&](int ks) {
             bf16x8 fx[4], fy[4];
             auto at = [&](int r) { return r * 128 + (((2 * ks + fhalf) ^ swz8s(r)) << 4); };
