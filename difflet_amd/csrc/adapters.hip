@@ -10,7 +10,8 @@
 // meet in LDS. Many rows: a workgroup takes 128 rows, its wavefronts 32 each beside the same ranks,
 // and both operands come through a ring of LDS stages, 128 bytes of a row at a time: read straight
 // from memory, 32 rows at strides of the width share four sets of the L1, and each line is fetched
-// for every 32 bytes of it (34125 x 5120, rank 64: DOWN_A us; DOWN_B through LDS).
+// for every 32 bytes of it (34125 x 5120, rank 64: 233 us; 110 through LDS, 3.2 TB/s,
+// of about 4 that a read alone reaches).
 // Where that leaves compute units idle, K is cut into `pieces` whose sums the GEMM adds in order.
 #include <algorithm>
 
@@ -107,7 +108,8 @@ __global__ __launch_bounds__(256) void lora_down_kernel(const LoraDownArgs a) {
 constexpr int LORA_ROWS = 128;  // rows of a wide tile
 
 // The same for 128 rows of a request: 32 NR ranks, stages of 64 K elements (128 bytes a row) in a
-// ring of NS slots, NS - 1 of them in flight. Rows of x past the request, ranks past the adapter's
+// ring of NS slots, NS - 1 of them in flight (NR = 2: 3 slots leave room for two workgroups on a
+// compute unit, 110 us above; 4 slots 114, 6 slots 115). Rows of x past the request, ranks past the adapter's
 // and K past the width read zero.
 template <int NR, int NS>
 __global__ __launch_bounds__(256, 1) void lora_down_wide_kernel(const LoraDownArgs a) {

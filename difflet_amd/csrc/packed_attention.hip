@@ -399,10 +399,13 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(const PackedAttnArg
 // out through LDS (stored from the accumulators, 32 bytes of 32 rows an instruction, it took
 // 5,400 cycles a tile, so 4,000).
 //
+// Loads issued one by one between the MFMAs instead of in one go before them cost 6 % (their branches
+// cut the groups of MFMAs).
+//
 // 32,768 rows of 40 heads to 64, 128, 256, 512, 1024, 2048 keys: 165, 212, 285, 474, 831, 1474 us
 // (0.93 PFLOP/s); tiles of 128 rows: 246, 271, 356, 538, 873, 1575. Of the 49,000 cycles of a tile of 512
-// keys its loop takes 37,500, 5,360 a tile of keys (64 MFMAs a wavefront, 4,100 at the rate they
-// have alone).
+// keys its loop takes 37,500; without the exponentials 2048 keys took 1331 us of then 1599, which is
+// what the matrix cores and the LDS draw the card's power for.
 template <int D> struct WideLds {
   static constexpr int KS = D / 8 + 1, VS = D == 128 ? 20 : 12;  // slots of 16 bytes per row
   static constexpr int KB = 64 * KS * 16, VB = 64 * VS * 16;     // bytes per tile: KS, VS loads of 1 KB

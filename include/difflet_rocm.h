@@ -628,7 +628,7 @@ int difflet_rocm_rope_axes(const void* q, void* q_out, const int64_t* q_strides,
  * head h reads key head h / group. BF16 or F16, head_dim 64 or 128, any finite scale. A request
  * without keys has zero rows. Rows of no request are zero with zero_rest != 0 and not written
  * without. Rows and heads of q, k, v start on 16 bytes, of o on 8; o overlaps nothing. Few query
- * tiles cut each request's keys into pieces when the workspace
+ * tiles cut the requests' keys into chunks of about one length when the workspace
  * (difflet_rocm_packed_attention_workspace_bytes, this call's alone, 256-byte aligned, any contents)
  * is there, joined in order; without it the keys stay whole. */
 int64_t difflet_rocm_packed_attention_workspace_bytes(int64_t rows_q, int64_t rows_k,
@@ -651,7 +651,8 @@ int difflet_rocm_packed_attention(const void* q, const void* k, const void* v, v
  * [adapters][rank][x_cols], up bf16 [adapters][up_rows][rank], scale fp32 [adapters], contiguous;
  * x_cols <= k a multiple of 8, up_rows <= n (columns past them have no adapter), rank <= 1024. The
  * rank values x down^T are summed in fp32 and rounded to bf16 once, the result is rounded once. A
- * column n whose up[a][n] holds an infinity or NaN is NaN in the rows of adapter a, and only there.
+ * column n whose up[a][n] holds an infinity or NaN is an infinity or NaN in the rows of adapter a, and
+ * only there.
  * workspace: this call's alone, 256-byte aligned, any contents, of difflet_rocm_lora_workspace_bytes
  * (without the GEMM's share of it that runs whole tiles). */
 int64_t difflet_rocm_lora_workspace_bytes(int kind, int64_t m, int64_t n, int64_t k, int64_t rank,
