@@ -230,3 +230,38 @@ def test_lora_linear_compiles(gpu):
 
     f = lambda x: lora_linear(x * 2, c["w"], c["b"], c["down"], c["up"], c["scale"], st, ids) + 1  # noqa: E731
     assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(c["x"]), f(c["x"]))
+
+
+@pytest.mark.parametrize("count", [62, 63, 64, 65])
+@pytest.mark.parametrize("length,n", [(5, 512), (41, 512), (300, 1024)])
+def test_lora_linear_around_a_wavefront_of_requests(gpu, count, length, n):
+    """Tiles of one request, of several and of more requests than a wavefront has lanes."""
+    rows = count * length + 3
+    c = case(gpu, rows, 256, n, 7, 24)
+    ids = [(5 * i) % 8 - 1 for i in range(count)]
+    check(run(c, [length] * count, ids, gpu, 2), exact(c, [length] * count, ids, first=2))
+
+
+@pytest.mark.parametrize("rank", [3, 8, 24, 72, 200])
+@pytest.mark.parametrize("k,n", [(512, 1024), (1024, 4096)])
+def test_lora_linear_tiles_that_end_with_a_request(gpu, k, n, rank):
+    """Requests that fill whole tiles, empty ones on their borders, tiles of no request before, between
+    and behind, in launches of few and of many tiles."""
+    lengths, ids = [256, 0, 0, 256, 512, 0, 2048, 256], [2, 0, 1, 1, -1, 2, 0, 5]
+    for first in (0, 512, 300):
+        c = case(gpu, first + sum(lengths) + 600, k, n, 3, rank, seed=first)
+        check(run(c, lengths, ids, gpu, first), exact(c, lengths, ids, first=first))
+
+
+def test_lora_linear_of_one_request_keeps_the_formula(gpu):
+    """Rows that all have an adapter with an infinity: it stays in its column; no gradient is made up."""
+    for rows in (40, 3000):
+        c = case(gpu, rows, 512, 512, 2, 16)
+        c["up"][1, 17, 2] = float("inf")
+        y = run(c, [rows], [1], gpu)
+        assert not bool(y[:, 17].isfinite().any())
+        y[:, 17] = 0
+        assert bool(y.isfinite().all())
+    x = c["x"].clone().requires_grad_()
+    with pytest.raises(RuntimeError):
+        run(dict(c, x=x), [rows], [1], gpu).sum().backward()

@@ -331,3 +331,29 @@ def test_packed_cross_attention_of_many_rows_graph_follows_new_lengths(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         check(out, exact(q, k, v, lengths, keys, 0.1))
+
+
+def test_packed_cross_attention_of_many_rows_past_32_bits(gpu):
+    """Rows of q and of the output and states so far apart that their offsets pass 32 bits."""
+    from difflet_amd import kernels
+
+    rows, h, d, keys = 17000, 8, 64, [140, 60]
+    g = torch.Generator(device=gpu).manual_seed(0)
+    q, o = (torch.empty(rows << 18, dtype=BF16, device=gpu).as_strided((rows, h, d), (1 << 18, d, 1))
+            for _ in range(2))
+    kv = torch.empty((sum(keys) << 23), dtype=BF16, device=gpu)
+    k, v = (kv.as_strided((sum(keys), h, d), (1 << 23, d, 1), i * h * d) for i in (0, 1))
+    for t in (q, k, v):
+        t.copy_(torch.randn(t.shape, generator=g, device=gpu))
+    lengths = [9000, 8000]
+    kernels.packed_attention(q, k, v, starts(lengths, gpu), starts(keys, gpu), scale=0.1, out=o)
+    check(o, exact(q, k, v, lengths, keys, 0.1))
+
+
+def test_packed_cross_attention_makes_up_no_gradient(gpu):
+    from difflet_amd.backends.rocm.ops_impl.attention import packed_cross_attention
+
+    q, k, v = case(gpu, BF16, [70], [20], 2, 2, 64)
+    q.requires_grad_()
+    with pytest.raises(RuntimeError):
+        packed_cross_attention(q, k, v, starts([70], gpu), starts([20], gpu)).sum().backward()

@@ -264,3 +264,16 @@ def test_packed_rows_operators_replay_in_a_graph(gpu):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_packed_rows_operators_make_up_no_gradient(gpu):
+    from difflet_amd.backends.rocm.ops_impl.embeddings import apply_rotary_axes
+    from difflet_amd.backends.rocm.ops_impl.norm import rms_norm_quantized
+
+    x, r, w = norm_case(gpu, BF16, 9, 256)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError):
+        rms_norm_quantized(x, w, 1e-6, residual=r)[2].float().sum().backward()
+    pos = torch.zeros(9, 1, dtype=torch.int32, device=gpu)
+    with pytest.raises(RuntimeError):
+        apply_rotary_axes(x.view(9, 2, 128), None, pos, (64,))[0].float().sum().backward()
