@@ -298,8 +298,8 @@ def _(x, cos, sin, law):
 
 # ---------------------------------------------------------------------------- packed requests
 # Called with single tokens, where a trip through the dispatcher (4 us) would be a fifth of the call:
-# in plain eager inference, which is what _inference() says, the implementations are called as they
-# are. Everything else goes to the custom_op, whose backward refuses.
+# in plain eager inference, which is what _inference() says, the kernels are called as they are.
+# Everything else goes to the custom_op, whose backward refuses.
 def _rms_norm_quant_impl(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
                          eps: float, mx: bool) -> tuple[Tensor, Tensor, Tensor]:
     """difflet_rocm_rms_norm_quant on x [rows, dim]: (codes, scales, x + residual, which is empty
@@ -323,8 +323,9 @@ _rms_norm_quant_op.register_fake(_rms_norm_quant_fake)
 
 def rms_norm_quant(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float,
                    mx: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """The third output has a meaning with a residual only."""
     if _inference(x, weight, residual):
-        return _rms_norm_quant_impl(x, weight, residual, eps, mx)
+        return kernels.rms_norm_quant(x, weight, eps, residual=residual, mx=mx)
     return _rms_norm_quant_op(x, weight, residual, eps, mx)
 
 
@@ -344,9 +345,10 @@ _rope_axes_op.register_fake(_rope_axes_fake)
 
 
 def rope_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, axes: list[int], theta: float,
-              halves: bool, shared: bool) -> tuple[Tensor, Tensor]:
+              halves: bool, shared: bool) -> tuple[Tensor, Optional[Tensor]]:
+    """The second output has a meaning with k only."""
     if _inference(q, k, positions):
-        return _rope_axes_impl(q, k, positions, axes, theta, halves, shared)
+        return kernels.rope_axes(q, k, positions, axes, theta=theta, halves=halves, shared=shared)
     return _rope_axes_op(q, k, positions, axes, theta, halves, shared)
 
 

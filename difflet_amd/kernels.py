@@ -1270,14 +1270,18 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
 
 @functools.lru_cache(maxsize=64)
 def _rope_pairs(axes: tuple, theta: float, shared: bool):
-    """Turns per position and axis of every rotated pair, as host arrays."""
+    """Turns per position and axis of every rotated pair, as host arrays, and the channels they turn."""
+    if not 1 <= len(axes) <= 8 or any(d < 2 or d % 2 for d in axes):
+        raise ValueError(f"rope_axes: 1 to 8 axes of an even number of channels each, got {axes}")
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"rope_axes: theta must be positive, got {theta}")
     turns, axis, total = [], [], sum(axes)
     for a, d in enumerate(axes):
         for j in range(d // 2):
             e = 2.0 * (len(axis) if shared else j) / (total if shared else d)
             turns.append(theta ** -e / (2.0 * math.pi))
             axis.append(a)
-    return (ctypes.c_double * len(turns))(*turns), (ctypes.c_uint8 * len(axis))(*axis)
+    return (ctypes.c_double * len(turns))(*turns), (ctypes.c_uint8 * len(axis))(*axis), total
 
 
 _POSITIONS = {torch.float32: _lib.F32, torch.int32: _lib.I32, torch.int64: -1}
@@ -1292,27 +1296,23 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     positions [batch or 1, seq, len(axes)] (int32, int64 or fp32): axis a turns axes[a] channels.
     q_out, k_out: where to write (the inputs may be given); new contiguous tensors without."""
     dev = _device_of(q, k, positions, q_out, k_out)
-    axes = tuple(int(d) for d in axes)
-    if not 1 <= len(axes) <= 8 or any(d < 2 or d % 2 for d in axes):
-        raise ValueError(f"rope_axes: 1 to 8 axes of an even number of channels each, got {axes}")
-    if not (math.isfinite(theta) and theta > 0):
-        raise ValueError(f"rope_axes: theta must be positive, got {theta}")
+    axes = tuple([int(d) for d in axes])
+    turns, axis, total = _rope_pairs(axes, float(theta), bool(shared))
     if q.dim() != 4 or q.dtype not in FLOAT_DTYPES:
         raise ValueError(f"rope_axes: q must be a bf16, fp16 or fp32 [batch, seq, heads, dim], got "
                          f"{q.dtype} {tuple(q.shape)}")
-    b, s, _, d = q.shape
-    if sum(axes) > d:
+    b, s, h, d = q.shape
+    if total > d:
         raise ValueError(f"rope_axes: axes {axes} turn more than the head's {d} channels")
-    if sum(axes) > 256:
+    if total > 256:
         raise NotImplementedError(f"rope_axes: axes {axes} turn more than 256 channels")
-    if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != (b, s)
-                          or k.shape[3] != d):
+    hk = 0 if k is None or k.dim() != 4 else k.shape[2]
+    if k is not None and (k.dtype != q.dtype or k.shape != (b, s, hk, d)):
         raise ValueError(f"rope_axes: k must be {q.dtype} [{b}, {s}, heads, {d}], got {k.dtype} "
                          f"{tuple(k.shape)}")
     if positions.dtype not in _POSITIONS:
         raise TypeError(f"rope_axes: positions must be int32, int64 or fp32, got {positions.dtype}")
-    if positions.dim() != 3 or positions.shape[0] not in (1, b) or \
-            positions.shape[1:] != (s, len(axes)):
+    if positions.shape not in ((b, s, len(axes)), (1, s, len(axes))):
         raise ValueError(f"rope_axes: positions must be [{b} or 1, {s}, {len(axes)}], got "
                          f"{tuple(positions.shape)}")
     positions = positions.contiguous()
@@ -1333,15 +1333,14 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
 
     q, q_out = prepared(q, q_out, "q_out")
     k, k_out = prepared(k, k_out, "k_out")
-    turns, axis = _rope_pairs(axes, float(theta), bool(shared))
     strides = _I64x12(*q.stride()[:3], *q_out.stride()[:3],
                       *(() if k is None else (*k.stride()[:3], *k_out.stride()[:3])))
     at = ctypes.addressof(strides)
     _launch(dev, "rope_axes", lib().difflet_rocm_rope_axes, q.data_ptr(), q_out.data_ptr(), at,
-            at + 24, q.shape[2], _p(k), _p(k_out), at + 48, at + 72, 0 if k is None else k.shape[2],
-            _DT[q.dtype], b, s, d, positions.data_ptr(), _POSITIONS[positions.dtype],
-            positions.stride(0) if positions.shape[0] > 1 else 0, len(axes), sum(axes) // 2, turns,
-            axis, int(halves))
+            at + 24, h, _p(k), _p(k_out), at + 48, at + 72, hk, _DT[q.dtype], b, s, d,
+            positions.data_ptr(), _POSITIONS[positions.dtype],
+            0 if positions.shape[0] == 1 else positions.stride(0), len(axes), total // 2, turns, axis,
+            int(halves))
     return q_out, k_out
 
 
