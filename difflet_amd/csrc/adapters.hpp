@@ -258,13 +258,7 @@ __device__ __forceinline__ void lora_stage(const LoraDev& L, int m0, int n0, int
   for (int i = 0; i < BN / RP; ++i) {
     const int n = n0 + i * RP + (tid >> 3);
     w[i] = u32x4{0u, 0u, 0u, 0u};
-    if (!on || n >= L.n || r8 >= L.rank) continue;
-    w[i] = lora_up8(L, a, n, r8);
-    if (lora_finite8(w[i])) {
-      const int c = n - n0;
-      atomicOr(&bad[s * (BN / 32) + (c >> 5)], 1u << (c & 31));
-      bad[-1] = 1u;
-    }
+    if (on && n < L.n && r8 < L.rank) w[i] = lora_up8(L, a, n, r8);
   }
   u32x4 x[BM / RP];
 #pragma unroll
@@ -283,6 +277,10 @@ __device__ __forceinline__ void lora_stage(const LoraDev& L, int m0, int n0, int
 #pragma unroll
   for (int i = 0; i < BN / RP; ++i) {
     const int r = i * RP + (tid >> 3);
+    if (lora_finite8(w[i])) {  // looked at after both operands' loads went out
+      atomicOr(&bad[s * (BN / 32) + (r >> 5)], 1u << (r & 31));
+      bad[-1] = 1u;
+    }
     *reinterpret_cast<u32x4*>(stage + (BM + r) * 128 + ((ch ^ swz(r)) << 4)) = w[i];
   }
   __syncthreads();
